@@ -444,6 +444,161 @@ int spl_sage_ring_segment(int rank, int world, int step, int64_t chunk, int64_t*
 int spl_sage_ring_forward(spl_sage* s, spl_sage_ring* r, spl_sage_tensor q, spl_sage_tensor k, spl_sage_tensor v,
                           spl_sage_tensor_mut out, const spl_sage_options* opts, void* nccl_comm);
 
+/* ---- Serving: after the prompt ----
+ * No counterpart in the reference, whose transformers see all their tokens at
+ * once.  What a decoder needs next to the projection and the prompt's
+ * attention: rotary positions anywhere in a long context, a paged KV cache in
+ * 4 bits, and attention over it for single tokens, drafted tokens and pieces
+ * of prompts.
+ *
+ * Conventions: tensors are [token][head][head_dim] views (the batch stride of
+ * spl_sage_tensor is not used), bf16 unless said otherwise, strides multiples
+ * of 8 elements, starting on 16 bytes.  Index arrays (positions, slots,
+ * q_start, kv_len, pages) are int32 on the device.  What only the device
+ * knows is checked there: an index out of range is left out as each call
+ * says, nothing is read or written outside the buffers, and the engine's error
+ * word (spl_sage_engine_status) gets SPL_SAGE_DEVERR_INDEX.  The calls enqueue
+ * on the engine's stream, need the engine's device to be the current one, and
+ * can be captured into a CUDA graph. */
+#define SPL_SAGE_DEVERR_INDEX 0x4u /* device error word: an index in device memory was out of range */
+
+/* The device an engine was made on. */
+int spl_sage_device(const spl_sage* s);
+
+/* Types of spl_sage_rope. */
+#define SPL_SAGE_BF16 0
+#define SPL_SAGE_F16 1
+#define SPL_SAGE_F32 2
+
+/* Rotary positions: channels 0 .. rot_dim - 1 of a head turn in pairs, the
+ * rest pass.  Pair p is channels (p, p + rot_dim/2), or with interleaved
+ * (2p, 2p + 1).  rot_dim: a multiple of 16 up to the head dim.  table: device
+ * f32 [positions][rot_dim/2][2] (cos, sin), on 16 bytes (spl_sage_rope_table). */
+typedef struct {
+    const float* table;
+    int64_t positions;
+    int32_t rot_dim;
+    int32_t interleaved;
+} spl_sage_rotary;
+
+/* How the angles of a longer context follow from base and position t: pair p
+ * turns by t * f(p), f(p) = base^(-2p/rot_dim), and
+ *   LINEAR  f / factor;
+ *   NTK     base * factor^(rot_dim / (rot_dim - 2)) in place of base;
+ *   YARN    f / factor for pairs that make fewer than `low` turns over the
+ *           original context, f for those that make more than `high`, blended
+ *           linearly in p between (whole pairs); cos and sin times `attention`
+ *           (0: 0.1 ln(factor) + 1);
+ *   BANDS   the same ends, blended linearly in the number of turns. */
+#define SPL_SAGE_ROPE_PLAIN 0
+#define SPL_SAGE_ROPE_LINEAR 1
+#define SPL_SAGE_ROPE_NTK 2
+#define SPL_SAGE_ROPE_YARN 3
+#define SPL_SAGE_ROPE_BANDS 4
+typedef struct {
+    int32_t kind;
+    int32_t reserved;
+    double factor;    /* 1 .. 1e6 */
+    int64_t original; /* the original context, YARN and BANDS */
+    double low, high; /* turns, YARN and BANDS: 0 < low < high (YARN usually 1 and 32, BANDS 1 and 4) */
+    double attention; /* YARN */
+} spl_sage_rope_scaling;
+
+/* A rotary table, computed in f64 and stored f32, in host memory: positions *
+ * rot_dim floats.  scaling NULL: plain.  With a plain scaling and rot_dim =
+ * head_dim it is spl_sage_rope_table_1d's. */
+int spl_sage_rope_table(double base, int rot_dim, int64_t positions, const spl_sage_rope_scaling* scaling,
+                        float* out);
+
+/* out = R(positions[t]) x on `heads` heads of `tokens` tokens, x and out of
+ * type dtype, in f32 with one rounding; backward: the transposed rotation,
+ * which takes the gradient of out to that of x.  out may be x (same data and
+ * strides), and must not overlap it otherwise.  A token whose position is not
+ * in the table is left as it was. */
+int spl_sage_rope(spl_sage* s, int dtype, int64_t tokens, int64_t heads, spl_sage_tensor x, spl_sage_tensor_mut out,
+                  const spl_sage_rotary* rotary, const int32_t* positions, int backward);
+
+/* The paged 4-bit cache: a pool of pages in the caller's memory, each of
+ * page_tokens (16, 32, 64 or 128) consecutive tokens of one sequence, page i at
+ * byte i * page_stride.  A page holds kv_heads blocks of
+ * spl_sage_kv4_block_bytes each:
+ *   K values u8 [page_tokens][D/2] (channel 2j in the low half of byte j, 2j + 1
+ *   in the high half), V values likewise, K parameters bf16
+ *   [page_tokens][D/64][2] (scale, zero), V parameters likewise.
+ * A value is zero + scale * n, n = 0 .. 15: one scale and zero per 64 channels
+ * of a token.  Slot i is token i % page_tokens of page i / page_tokens. */
+typedef struct {
+    void* data;          /* on 16 bytes */
+    int64_t pages;       /* pages * page_tokens < 2^31 */
+    int64_t page_stride; /* bytes, a multiple of 16, at least kv_heads blocks */
+    int32_t page_tokens;
+    int32_t kv_heads;
+} spl_sage_kv4;
+
+/* Bytes of one page of one KV head: page_tokens * (D + D/8); 0 where the head
+ * dim or page size is not supported. */
+int64_t spl_sage_kv4_block_bytes(int head_dim, int page_tokens);
+
+/* Appends `tokens` tokens: K (rotated by its position) and V of kv_heads heads
+ * are quantised and written to slots[t].  zero = bf16(min), scale = bf16((max -
+ * min) * (1/15)) over the 64 channels, n = rint((x - zero) / scale) in 0 .. 15,
+ * all in f32 from the rotated channels: the bytes are defined to the bit.  A
+ * group with a NaN or an infinity, or whose range passes bf16's, is stored as
+ * NaN; one with a scale below 2^-100 as its zero.  rotary NULL (positions NULL
+ * too): K as it is.  q_heads > 0: Q rotated likewise into q_out (bf16), which
+ * may be Q (same data and strides) and must not overlap an input otherwise.
+ * slots[t] < 0: the token is not cached (its Q is rotated all the same); a slot
+ * or position out of range: the token is left out.  A slot named twice in one
+ * call is left holding a mix of the two tokens. */
+int spl_sage_kv4_append(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, spl_sage_tensor k, spl_sage_tensor v,
+                        const int32_t* slots, const spl_sage_rotary* rotary, const int32_t* positions,
+                        int64_t q_heads, spl_sage_tensor q, spl_sage_tensor_mut q_out);
+
+/* The cached values at `slots`, zero + scale * n rounded to bf16, into k and v
+ * [tokens][kv_heads][D] (e.g. a cached prefix for a dense kernel).  slots[t] <
+ * 0: zeros; out of range: the rows are left as they were. */
+int spl_sage_kv4_read(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, const int32_t* slots,
+                      spl_sage_tensor_mut k, spl_sage_tensor_mut v);
+
+/* Scratch of spl_sage_kv4_attend (partial outputs of sequences that are split
+ * over the GPU), for any shape on this engine's GPU and head dim.  Calls that
+ * share one must not run at the same time: use one per stream, and one per
+ * captured graph if graphs are replayed side by side. */
+typedef struct spl_sage_kv4_ws spl_sage_kv4_ws;
+int spl_sage_kv4_ws_create(spl_sage* s, spl_sage_kv4_ws** out);
+void spl_sage_kv4_ws_destroy(spl_sage_kv4_ws* ws);
+int64_t spl_sage_kv4_ws_bytes(const spl_sage_kv4_ws* ws);
+
+typedef struct {
+    int64_t batch;     /* sequences */
+    int64_t heads;     /* query heads, a multiple of the cache's kv_heads */
+    int64_t tokens;    /* query rows in q and out, all sequences together */
+    int64_t max_q;     /* no sequence has more query tokens in this call */
+    int64_t max_pages; /* page ids per sequence */
+    int32_t causal;
+    int32_t window;    /* 0: none */
+} spl_sage_kv4_shape;
+
+/* out = softmax(scale * Q K^T + mask) V over the cache.  Sequence b has kv_len[b]
+ * cached tokens, in pages[b][0 ..] (max_pages ids a row; ids behind the last
+ * page needed are not looked at), and query tokens q_start[b] ..
+ * q_start[b + 1] - 1 of q (q_start [batch + 1], ascending; NULL: one each, row
+ * b), which are its last: query i of n sits at position kv_len - n + i.
+ * causal: it sees the keys up to its own position (none at a negative one),
+ * otherwise all kv_len; window w > 0: only keys after its position - w (and
+ * pages wholly before every query's window are not looked at).  A query that
+ * sees no key gives zeros and an lse of -infinity.  q is bf16 and already
+ * rotated; K and V are the exact cached values; scores, statistics and sums
+ * are f32, a probability times its V scale is rounded to bf16 once.  opts: the
+ * softmax scale (default 1 / sqrt(head_dim)); NULL = default.  out must not
+ * overlap q; rows of no sequence are left as they were.  lse: f32
+ * [tokens][heads], the natural logarithm of each row's softmax denominator, or
+ * NULL.  A bad page id, length or q_start leaves the rows of its sequence
+ * unspecified. */
+int spl_sage_kv4_attend(spl_sage* s, spl_sage_kv4_ws* ws, const spl_sage_kv4* cache, const spl_sage_kv4_shape* shape,
+                        spl_sage_tensor q, const int32_t* q_start, const int32_t* kv_len, const int32_t* pages,
+                        const spl_sage_options* opts, spl_sage_tensor_mut out, float* lse);
+
 /* Tensor-core peak probe (the analog of the reference's sage_peak kernels,
  * platform/spl-nn/cuda/sage_peak.cu, measured by src/sage/tests.rs:758-794):
  * one CTA per SM issues `iters` x 4 back-to-back tcgen05.mma of M=128, N=n

@@ -24,7 +24,7 @@ from dataclasses import dataclass, field
 __all__ = [
     "QGROUP", "QTILE", "KBLOCK", "FP8_MAX", "PV16_V_RANGE", "SageError", "Tile", "PvAccum", "Config", "Strides",
     "Shape", "FrameLayout", "KvMerge", "Options", "QkNorm", "Plan", "Tensor", "TensorMut", "Workspace",
-    "SageAttention", "flops", "library_path",
+    "SageAttention", "flops", "library_path", "RopeScaling", "Rotary", "Kv4Cache", "Kv4Workspace",
 ]
 
 QGROUP = 16      # mod.rs:71
@@ -92,6 +92,28 @@ class _Plan(ctypes.Structure):
     _fields_ = [("tq_pad", ctypes.c_int64), ("tk", ctypes.c_int64), ("tk_pad", ctypes.c_int64)]
 
 
+class _Rotary(ctypes.Structure):
+    _fields_ = [("table", ctypes.c_void_p), ("positions", ctypes.c_int64), ("rot_dim", ctypes.c_int32),
+                ("interleaved", ctypes.c_int32)]
+
+
+class _RopeScaling(ctypes.Structure):
+    _fields_ = [("kind", ctypes.c_int32), ("reserved", ctypes.c_int32), ("factor", ctypes.c_double),
+                ("original", ctypes.c_int64), ("low", ctypes.c_double), ("high", ctypes.c_double),
+                ("attention", ctypes.c_double)]
+
+
+class _Kv4(ctypes.Structure):
+    _fields_ = [("data", ctypes.c_void_p), ("pages", ctypes.c_int64), ("page_stride", ctypes.c_int64),
+                ("page_tokens", ctypes.c_int32), ("kv_heads", ctypes.c_int32)]
+
+
+class _Kv4Shape(ctypes.Structure):
+    _fields_ = [("batch", ctypes.c_int64), ("heads", ctypes.c_int64), ("tokens", ctypes.c_int64),
+                ("max_q", ctypes.c_int64), ("max_pages", ctypes.c_int64), ("causal", ctypes.c_int32),
+                ("window", ctypes.c_int32)]
+
+
 EXPORTS = [
     "spl_sage_default_config", "spl_sage_default_options", "spl_sage_create", "spl_sage_destroy",
     "spl_sage_workspace_create", "spl_sage_ws_destroy", "spl_sage_ws_bytes", "spl_sage_ws_plan", "spl_sage_prepare",
@@ -104,6 +126,9 @@ EXPORTS = [
     "spl_sage_linear_fp8", "spl_sage_gemm_pairs", "spl_sage_ring_create", "spl_sage_ring_destroy",
     "spl_sage_ring_forward", "spl_sage_plan_new", "spl_sage_wait_selftest", "spl_sage_ring_segment",
     "spl_sage_kv_create_gathered", "spl_sage_cp_attend_gathered", "spl_sage_ring_schedule",
+    "spl_sage_device", "spl_sage_rope_table", "spl_sage_rope", "spl_sage_kv4_block_bytes", "spl_sage_kv4_append",
+    "spl_sage_kv4_read", "spl_sage_kv4_ws_create", "spl_sage_kv4_ws_destroy", "spl_sage_kv4_ws_bytes",
+    "spl_sage_kv4_attend",
 ]
 
 # spl_sage_cp_attend flags
@@ -171,6 +196,21 @@ def lib() -> ctypes.CDLL:
         L.spl_sage_cp_quantize_kv.argtypes = [P, P, _Tensor, _Tensor, ctypes.POINTER(_Options), P, ctypes.c_int64, P]
         L.spl_sage_cp_attend.argtypes = [P, P, P] + [ctypes.c_int64] * 4 + [I, P, P]
         L.spl_sage_cp_finish.argtypes = [P, P, P, _Tensor]
+        I64 = ctypes.c_int64
+        L.spl_sage_device.argtypes = [P]
+        L.spl_sage_rope_table.argtypes = [ctypes.c_double, I, I64, ctypes.POINTER(_RopeScaling), P]
+        L.spl_sage_rope.argtypes = [P, I, I64, I64, _Tensor, _Tensor, ctypes.POINTER(_Rotary), P, I]
+        L.spl_sage_kv4_block_bytes.restype = I64
+        L.spl_sage_kv4_block_bytes.argtypes = [I, I]
+        L.spl_sage_kv4_append.argtypes = [P, ctypes.POINTER(_Kv4), I64, _Tensor, _Tensor, P, ctypes.POINTER(_Rotary),
+                                          P, I64, _Tensor, _Tensor]
+        L.spl_sage_kv4_read.argtypes = [P, ctypes.POINTER(_Kv4), I64, P, _Tensor, _Tensor]
+        L.spl_sage_kv4_ws_create.argtypes = [P, ctypes.POINTER(P)]
+        L.spl_sage_kv4_ws_destroy.argtypes = [P]
+        L.spl_sage_kv4_ws_bytes.restype = I64
+        L.spl_sage_kv4_ws_bytes.argtypes = [P]
+        L.spl_sage_kv4_attend.argtypes = [P, P, ctypes.POINTER(_Kv4), ctypes.POINTER(_Kv4Shape), _Tensor, P, P, P,
+                                          ctypes.POINTER(_Options), _Tensor, P]
         L.spl_sage_flops.restype = ctypes.c_double
         L.spl_sage_flops.argtypes = [P]
         L.spl_sage_last_error.restype = ctypes.c_char_p
@@ -416,6 +456,7 @@ class SageAttention:
         self.config = cfg
         self.stream = stream
         self.reserved_sms = 0
+        self.device = lib().spl_sage_device(h)
 
     @staticmethod
     def new(stream, head_dim: int) -> "SageAttention":
@@ -592,6 +633,104 @@ class SageAttention:
 
     def cp_finish(self, ws: Workspace, acc, out: Tensor):
         _check(lib().spl_sage_cp_finish(self._h, ws._h, ctypes.c_void_p(acc.data_ptr()), out._c()))
+
+    # ------------------------------------------------------------ serving
+    # (no counterpart in the reference; splsage.h has the conventions)
+
+    def _rows(self, what: str, t, dtypes, tokens: int, heads: int) -> _Tensor:
+        """A CUDA tensor [tokens][heads][head_dim] of this engine's device as a view."""
+        st = t.stride()
+        if not t.is_cuda or t.device.index != self.device or t.dtype not in dtypes:
+            raise SageError(ERR_INVALID, f"{what} must be a tensor of {' or '.join(str(x) for x in dtypes)} on device "
+                                         f"{self.device}, got {t.dtype} on {t.device}")
+        if tuple(t.shape) != (tokens, heads, self.head_dim) or (st[2] != 1 and t.numel()):
+            raise SageError(ERR_INVALID, f"{what} must be [{tokens}][{heads}][{self.head_dim}] with channels "
+                                         f"contiguous, got {tuple(t.shape)} with strides {st}")
+        if min(st) < 0:
+            raise SageError(ERR_INVALID, f"{what} has a negative stride")
+        # a stride of an axis of length 1 is never used
+        a = st[0] if tokens > 1 else 0
+        b = st[1] if heads > 1 else 0
+        return _Tensor(t.data_ptr(), (tokens - 1) * a + (heads - 1) * b + self.head_dim if t.numel() else 0, 0, a, b)
+
+    def _index(self, what: str, t, shape: tuple) -> int:
+        """The address of an int32 CUDA array of this engine's device."""
+        import torch
+        if (not t.is_cuda or t.device.index != self.device or t.dtype != torch.int32 or tuple(t.shape) != shape
+                or not t.is_contiguous()):
+            raise SageError(ERR_INVALID, f"{what} must be a contiguous int32 tensor {list(shape)} on device "
+                                         f"{self.device}, got {t.dtype} {list(t.shape)} on {t.device}")
+        return t.data_ptr()
+
+    def rope(self, x, out, rotary: "Rotary", positions, *, backward: bool = False):
+        """out = R(positions) x for x [tokens][heads][head_dim] in bf16, f16 or
+        f32 (spl_sage_rope); out of the same shape and type may be x.
+        backward: the transposed rotation, the gradient's."""
+        types = _rope_types()
+        t, h = x.shape[0], x.shape[1]
+        cx, co = self._rows("x", x, tuple(types), t, h), self._rows("output", out, (x.dtype,), t, h)
+        _check(lib().spl_sage_rope(self._h, types[x.dtype], t, h, cx, co, ctypes.byref(rotary._c(self)),
+                                   self._index("positions", positions, (t,)), int(backward)))
+
+    def kv4_append(self, cache: "Kv4Cache", k, v, slots, *, rotary: "Rotary | None" = None, positions=None, q=None,
+                   q_out=None):
+        """Tokens into the 4-bit cache (spl_sage_kv4_append): k and v bf16
+        [tokens][kv_heads][head_dim] at slots (int32 [tokens], -1: not
+        cached), K rotated by positions where a rotary is given; q bf16
+        [tokens][heads][head_dim] is rotated into q_out on the way."""
+        import torch
+        bf, t, c = (torch.bfloat16,), k.shape[0], cache._c(self)
+        ck, cv = self._rows("K", k, bf, t, c.kv_heads), self._rows("V", v, bf, t, c.kv_heads)
+        if (q is None) != (q_out is None):
+            raise SageError(ERR_INVALID, "Q and its output are given together, or neither")
+        if (rotary is None) != (positions is None):
+            raise SageError(ERR_INVALID, "a rotary and positions are given together, or neither")
+        hq = 0 if q is None else q.shape[1]
+        cq = _Tensor() if q is None else self._rows("Q", q, bf, t, hq)
+        co = _Tensor() if q is None else self._rows("Q output", q_out, bf, t, hq)
+        _check(lib().spl_sage_kv4_append(self._h, ctypes.byref(c), t, ck, cv, self._index("slots", slots, (t,)),
+                                         None if rotary is None else ctypes.byref(rotary._c(self)),
+                                         None if positions is None else self._index("positions", positions, (t,)),
+                                         hq, cq, co))
+
+    def kv4_read(self, cache: "Kv4Cache", slots, k, v):
+        """The cached values at slots into k and v, bf16
+        [tokens][kv_heads][head_dim] (spl_sage_kv4_read)."""
+        import torch
+        bf, t, c = (torch.bfloat16,), slots.shape[0], cache._c(self)
+        ck, cv = self._rows("K", k, bf, t, c.kv_heads), self._rows("V", v, bf, t, c.kv_heads)
+        _check(lib().spl_sage_kv4_read(self._h, ctypes.byref(c), t, self._index("slots", slots, (t,)), ck, cv))
+
+    def kv4_workspace(self) -> "Kv4Workspace":
+        """Scratch of kv4_attend: one per stream (spl_sage_kv4_ws_create)."""
+        return Kv4Workspace(self)
+
+    def kv4_attend(self, ws: "Kv4Workspace", cache: "Kv4Cache", q, out, pages, kv_len, *, q_start=None,
+                   max_q: int = 1, causal: bool = True, window: int = 0, softmax_scale: float | None = None, lse=None):
+        """Attention of q bf16 [tokens][heads][head_dim] over the 4-bit cache
+        (spl_sage_kv4_attend): pages int32 [batch][max_pages], kv_len int32
+        [batch], q_start int32 [batch + 1] (None: one query per sequence), at
+        most max_q queries a sequence; writes out and, where given, lse f32
+        [tokens][heads]."""
+        import torch
+        bf, t, h, c, b = (torch.bfloat16,), q.shape[0], q.shape[1], cache._c(self), kv_len.shape[0]
+        cq, co = self._rows("Q", q, bf, t, h), self._rows("output", out, bf, t, h)
+        if lse is not None and (not lse.is_cuda or lse.device.index != self.device or lse.dtype != torch.float32
+                                or tuple(lse.shape) != (t, h) or not lse.is_contiguous()):
+            raise SageError(ERR_INVALID, f"lse must be a contiguous f32 tensor [{t}][{h}] on device {self.device}")
+        if pages.dim() != 2:
+            raise SageError(ERR_INVALID, f"pages must be [batch][max_pages], got {list(pages.shape)}")
+        if not 0 <= window <= 1 << 30:  # the struct's field would wrap
+            raise SageError(ERR_INVALID, f"a window of {window} keys")
+        sh = _Kv4Shape(b, h, t, max_q, pages.shape[1], int(causal), window)
+        opts = None
+        if softmax_scale is not None:
+            opts = ctypes.byref(Options(softmax_scale=softmax_scale)._c())
+        _check(lib().spl_sage_kv4_attend(self._h, ws._h, ctypes.byref(c), ctypes.byref(sh), cq,
+                                         None if q_start is None else self._index("q_start", q_start, (b + 1,)),
+                                         self._index("kv_len", kv_len, (b,)),
+                                         self._index("pages", pages, (b, pages.shape[1])), opts, co,
+                                         None if lse is None else lse.data_ptr()))
 
     def status(self, ws: Workspace) -> int:
         """Reads (and clears) the device error word; raises on a kernel error."""
@@ -798,6 +937,147 @@ class RopeTable:
         """Llama-style 1-D positions 0..positions-1, frequency
         base^(-p/(D/2)) for pair p (spl_sage_rope_table_1d)."""
         return cls(RopeLayout.one_d(head_dim), rope_table_1d(base, head_dim, positions))
+
+
+_ROPE_TYPES = None
+
+
+def _rope_types() -> dict:
+    """torch types of SageAttention.rope -> SPL_SAGE_BF16, _F16, _F32."""
+    global _ROPE_TYPES
+    if _ROPE_TYPES is None:
+        import torch
+        _ROPE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+    return _ROPE_TYPES
+
+
+@dataclass(frozen=True)
+class RopeScaling:
+    """How a longer context's angles follow from the base
+    (spl_sage_rope_scaling): RopeScaling.linear(4.0), .ntk(4.0),
+    .yarn(4.0, 8192), .bands(8.0, 8192)."""
+    kind: int = 0
+    factor: float = 1.0
+    original: int = 0
+    low: float = 1.0
+    high: float = 32.0
+    attention: float = 0.0
+
+    @staticmethod
+    def linear(factor: float) -> "RopeScaling":
+        return RopeScaling(1, factor)
+
+    @staticmethod
+    def ntk(factor: float) -> "RopeScaling":
+        return RopeScaling(2, factor)
+
+    @staticmethod
+    def yarn(factor: float, original: int, low: float = 1.0, high: float = 32.0,
+             attention: float = 0.0) -> "RopeScaling":
+        return RopeScaling(3, factor, original, low, high, attention)
+
+    @staticmethod
+    def bands(factor: float, original: int, low: float = 1.0, high: float = 4.0) -> "RopeScaling":
+        return RopeScaling(4, factor, original, low, high)
+
+
+def rope_table(base: float, rot_dim: int, positions: int, scaling: RopeScaling | None = None):
+    """cos and sin of positions 0 .. positions - 1, f32 numpy
+    [positions][rot_dim/2][2] (spl_sage_rope_table)."""
+    import numpy as np
+    if positions <= 0 or rot_dim <= 0:  # before the array is made
+        raise SageError(ERR_INVALID, "rope_table: bad arguments")
+    out = np.empty((positions, rot_dim // 2, 2), np.float32)
+    s = scaling or RopeScaling()
+    c = _RopeScaling(s.kind, 0, s.factor, s.original, s.low, s.high, s.attention)
+    _check(lib().spl_sage_rope_table(base, rot_dim, positions, ctypes.byref(c), out.ctypes.data_as(ctypes.c_void_p)))
+    return out
+
+
+class Rotary:
+    """A rotary table on the device (f32 [positions][rot_dim/2][2], from
+    rope_table) with the layout of its pairs: channels (p, p + rot_dim/2), or
+    (2p, 2p + 1) where interleaved (spl_sage_rotary)."""
+
+    def __init__(self, table, rot_dim: int, interleaved: bool = False):
+        import torch
+        if (not table.is_cuda or table.dtype != torch.float32 or not table.is_contiguous() or table.dim() != 3
+                or tuple(table.shape[1:]) != (rot_dim // 2, 2)):
+            raise SageError(ERR_INVALID, f"a rotary table is a contiguous f32 CUDA tensor [positions][{rot_dim // 2}]"
+                                         f"[2], got {table.dtype} {list(table.shape)} on {table.device}")
+        self.table, self.rot_dim, self.interleaved = table, rot_dim, interleaved
+        self._struct = _Rotary(table.data_ptr(), table.shape[0], rot_dim, int(interleaved))
+
+    def _c(self, eng: "SageAttention") -> _Rotary:
+        if self.table.device.index != eng.device:
+            raise SageError(ERR_INVALID, f"the rotary table is on {self.table.device}, the engine on device {eng.device}")
+        return self._struct
+
+
+class Kv4Cache:
+    """A pool of pages of 4-bit keys and values (spl_sage_kv4): pool uint8
+    [pages][kv_heads][Kv4Cache.block_bytes(head_dim, page_tokens)], blocks
+    contiguous; a view of every second page, say, is fine."""
+
+    def __init__(self, pool, page_tokens: int, head_dim: int):
+        import torch
+        block = Kv4Cache.block_bytes(head_dim, page_tokens)
+        st = pool.stride()
+        if (not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != block or st[2] != 1
+                or (pool.shape[1] > 1 and st[1] != block)):
+            raise SageError(ERR_INVALID, f"a cache pool is a uint8 CUDA tensor [pages][kv_heads][{block}] with "
+                                         f"contiguous pages, got {pool.dtype} {list(pool.shape)} with strides {st} on "
+                                         f"{pool.device}")
+        self.pool, self.page_tokens, self.head_dim = pool, page_tokens, head_dim
+        pages, heads = pool.shape[0], pool.shape[1]
+        stride = st[0] if pages > 1 else heads * block
+        self._struct = _Kv4(pool.data_ptr(), pages, stride, page_tokens, heads)
+
+    @staticmethod
+    def block_bytes(head_dim: int, page_tokens: int) -> int:
+        """Bytes of one page of one KV head."""
+        n = lib().spl_sage_kv4_block_bytes(head_dim, page_tokens)
+        if not n:
+            raise SageError(ERR_INVALID, f"no 4-bit cache for head dim {head_dim} and pages of {page_tokens} tokens: "
+                                         "64 or 128, and 16, 32, 64 or 128")
+        return n
+
+    @staticmethod
+    def empty(pages: int, kv_heads: int, page_tokens: int, head_dim: int) -> "Kv4Cache":
+        """A pool of zeros on the current device."""
+        import torch
+        block = Kv4Cache.block_bytes(head_dim, page_tokens)
+        return Kv4Cache(torch.zeros(pages, kv_heads, block, dtype=torch.uint8, device="cuda"), page_tokens, head_dim)
+
+    def _c(self, eng: "SageAttention") -> _Kv4:
+        if self.head_dim != eng.head_dim or self.pool.device.index != eng.device:
+            raise SageError(ERR_INVALID, f"the cache is for head dim {self.head_dim} on {self.pool.device}, the engine "
+                                         f"for {eng.head_dim} on device {eng.device}")
+        return self._struct
+
+
+class Kv4Workspace:
+    """Scratch of SageAttention.kv4_attend (spl_sage_kv4_ws_create)."""
+
+    def __init__(self, eng: "SageAttention"):
+        self._h = None
+        h = ctypes.c_void_p()
+        _check(lib().spl_sage_kv4_ws_create(eng._h, ctypes.byref(h)))
+        self._h = h
+
+    def bytes(self) -> int:
+        return int(lib().spl_sage_kv4_ws_bytes(self._h))
+
+    def close(self):
+        if self._h:
+            lib().spl_sage_kv4_ws_destroy(self._h)
+            self._h = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
 
 
 def flops(plan: Plan, head_dim: int) -> float:

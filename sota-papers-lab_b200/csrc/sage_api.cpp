@@ -14,7 +14,11 @@
 #include <string>
 
 #include "../../include/splsage.h"
+#include "sage_host.h"
 #include "sage_kernels.h"
+
+using sp::cuda_fail;
+using sp::fail;
 
 namespace {
 
@@ -24,20 +28,6 @@ constexpr float PV16_V_RANGE = 2.25f;   // mod.rs:185
 constexpr int LN_Q = 1, LN_K = 2, SMOOTH_K = 4, SMOOTH_V = 8;
 
 thread_local std::string g_last_error;
-
-int fail(int code, const char* fmt, ...) {
-    char buf[1024];
-    va_list ap;
-    va_start(ap, fmt);
-    vsnprintf(buf, sizeof buf, fmt, ap);
-    va_end(ap);
-    g_last_error = buf;
-    return code;
-}
-
-int cuda_fail(cudaError_t e, const char* what) {
-    return fail(SPL_SAGE_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
-}
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
@@ -100,16 +90,19 @@ bool fits_i32(int64_t v) { return v >= 0 && v <= 0x7fffffffLL; }
 
 }  // namespace
 
-struct spl_sage {
-    cudaStream_t stream;
-    int head_dim;
-    spl_sage_config config;
-    int device;
-    int sm_count;
-    int reserved_sms;  // SMs the persistent kernels leave free (spl_sage_reserve_sms)
-    int gemm_pairs;    // GEMMs on SM pairs (spl_sage_gemm_pairs)
-    uint32_t* err;     // device error word of the calls that run without a workspace
-};
+int sp::fail(int code, const char* fmt, ...) {
+    char buf[1024];
+    va_list ap;
+    va_start(ap, fmt);
+    vsnprintf(buf, sizeof buf, fmt, ap);
+    va_end(ap);
+    g_last_error = buf;
+    return code;
+}
+
+int sp::cuda_fail(cudaError_t e, const char* what) {
+    return fail(SPL_SAGE_ERR_CUDA, "%s: %s (%s)", what, cudaGetErrorString(e), cudaGetErrorName(e));
+}
 
 namespace {
 // The CTA cap of a persistent kernel that leaves `reserved` SMs free (0: one

@@ -1,0 +1,733 @@
+"""The serving operators on the GPU against plain 64-bit forms: rotary
+positions (both layouts, part of the head, three types, the gradient), tokens
+into and out of the paged 4-bit cache (to the bit), attention over it (ragged
+batches, one token to pieces of prompts, every mask), the way they are used
+together, and calls at their edges.
+
+Tolerances count the roundings: half a step of the output's type (bf16 2^-8,
+f16 2^-11, f32 2^-24 relative), for attention also the one rounding to bf16
+of a probability times its V scale, and f32 sums."""
+import importlib
+import math
+
+import numpy as np
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+sage = importlib.import_module("sota-papers-lab_b200")
+
+DEV = "cuda"
+HALF = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0 ** -24}
+
+
+@pytest.fixture(scope="module")
+def engines():
+    made = {d: sage.SageAttention(torch.cuda.current_stream(), d) for d in (64, 128)}
+    made.update({("ws", d): made[d].kv4_workspace() for d in (64, 128)})
+    yield made
+    for d in (64, 128):
+        made[d].engine_status()
+
+
+def gen(seed):
+    return torch.Generator(device=DEV).manual_seed(seed)
+
+
+def rand(g, *shape, dtype=torch.bfloat16):
+    return torch.randn(*shape, generator=g, device=DEV).to(dtype)
+
+
+def table(rot, n, scaling=None):
+    return torch.from_numpy(sage.rope_table(10000.0, rot, n, scaling)).to(DEV)
+
+
+def ints(x):
+    return torch.as_tensor(x, dtype=torch.int32, device=DEV)
+
+
+# ---------------------------------------------------------------- rotary positions
+
+def rotate64(x, tab, pos, rot, inter, back=False):
+    cs = tab.double()[pos.long()][:, None]
+    c, s = cs[..., 0], cs[..., 1] * (-1 if back else 1)
+    y = x.double().clone()
+    i = torch.arange(rot // 2, device=DEV)
+    a, b = (2 * i, 2 * i + 1) if inter else (i, i + rot // 2)
+    xa, xb = x.double()[..., a], x.double()[..., b]
+    y[..., a], y[..., b] = xa * c - xb * s, xb * c + xa * s
+    return y
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+@pytest.mark.parametrize("d,rot,inter", [(64, 64, False), (64, 32, True), (128, 128, False), (128, 128, True),
+                                         (128, 96, False), (128, 16, True), (64, 48, False)])
+@pytest.mark.parametrize("tokens,heads", [(1, 1), (7, 5), (1500, 9)])
+def test_rope(engines, dtype, d, rot, inter, tokens, heads):
+    g = gen(1)
+    tab = table(rot, 3000, sage.RopeScaling.yarn(4.0, 1024))
+    pos = torch.randint(0, 3000, (tokens,), generator=g, device=DEV, dtype=torch.int32)
+    pos[-1] = 2999
+    wide = rand(g, tokens, heads + 3, d, dtype=dtype)  # heads of a wider row
+    x = wide[:, 2:2 + heads]
+    for back in (False, True):
+        out = torch.full((heads, tokens, d), 7.0, dtype=dtype, device=DEV).transpose(0, 1)  # head-major
+        engines[d].rope(x, out, sage.Rotary(tab, rot, inter), pos, backward=back)
+        want = rotate64(x, tab, pos, rot, inter, back)
+        # three f32 roundings of terms no larger than |x| * 1.2, then the type's
+        tol = HALF[dtype] * want.abs() + 3 * 2.0 ** -24 * 1.2 * x.double().abs().amax() + 2.0 ** -25
+        assert ((out.double() - want).abs() <= tol).all()
+        assert torch.equal(out[..., rot:], x[..., rot:])
+        keep = wide.clone()
+        engines[d].rope(x, x, sage.Rotary(tab, rot, inter), pos, backward=back)  # in place
+        assert torch.equal(x, out) and torch.equal(wide[:, :2], keep[:, :2]) and torch.equal(wide[:, 2 + heads:],
+                                                                                               keep[:, 2 + heads:])
+        wide.copy_(keep)
+    engines[d].engine_status()
+
+
+def test_rope_gradient_is_the_transposed_rotation(engines):
+    """<R x, w> differs by <e, R^T w> when x moves by e (exactly, being linear), f32 rounding aside."""
+    g, d, rot = gen(2), 128, 64
+    tab, pos = table(rot, 50, sage.RopeScaling.yarn(4.0, 16)), ints([0, 3, 49, 17])
+    x, w, e = (rand(g, 4, 3, d, dtype=torch.float32) for _ in range(3))
+    r = sage.Rotary(tab, rot, True)
+    y0, y1, back = (torch.empty_like(x) for _ in range(3))
+    engines[d].rope(x, y0, r, pos)
+    engines[d].rope(x + e, y1, r, pos)
+    engines[d].rope(w, back, r, pos, backward=True)
+    left = ((y1.double() - y0.double()) * w.double()).sum()
+    right = (((x + e).double() - x.double()) * back.double()).sum()
+    n = x.numel()
+    # each element is off by a few f32 roundings of numbers below 16; they add up at most like n of them
+    assert (left - right).abs() <= n * 8 * 2.0 ** -24 * 16 * float(w.abs().max())
+    want = rotate64(w, tab, pos, rot, True, True)
+    assert (back.double() - want).abs().max() <= 4 * 2.0 ** -24 * 1.2 * float(w.abs().max())
+
+
+def test_rope_positions_out_of_the_table(engines):
+    eng, g = engines[64], gen(3)
+    x, tab = rand(g, 5, 2, 64), table(64, 10)
+    out = torch.full_like(x, 3.0)
+    eng.rope(x, out, sage.Rotary(tab, 64), ints([0, -1, 9, 10, 2**31 - 1]))
+    assert (out[[1, 3, 4]] == 3.0).all() and (out[[0, 2]] != 3.0).any()
+    with pytest.raises(sage.SageError):
+        eng.engine_status()
+    eng.engine_status()  # cleared
+
+
+# ---------------------------------------------------------------- the cache
+
+def quantise(x):
+    """The stored form of f32 rows [..., D], by numpy's IEEE f32 operations:
+    n uint8 [..., D], scale and zero as f32 [..., D/64]."""
+    x = x.reshape(*x.shape[:-1], -1, 64)
+    bf = lambda v: torch.from_numpy(np.ascontiguousarray(v)).bfloat16().float().numpy()  # noqa: E731
+    with np.errstate(all="ignore"):
+        lo, hi = x.min(-1), x.max(-1)
+        rng = (hi - lo).astype(np.float32)
+        zero, scale = bf(lo), bf(rng * np.float32(1.0 / 15.0))
+        bad = ~(np.isfinite(x).all(-1) & np.isfinite(rng) & np.isfinite(zero) & np.isfinite(scale))
+        flat = scale < np.float32(2.0 ** -100)
+        scale[flat] = 0
+        n = np.rint((x - zero[..., None]) / scale[..., None])
+        n[np.broadcast_to((bad | flat)[..., None], n.shape)] = 0
+        n = np.clip(n, 0, 15).astype(np.uint8)
+    scale[bad] = zero[bad] = np.nan
+    return n.reshape(*n.shape[:-2], -1), scale, zero
+
+
+def parts(pool, page, d):
+    """Views of a pool (numpy uint8): K and V bytes [pages][heads][P][D/2], K
+    and V parameter bits uint16 [pages][heads][P][D/64][2]."""
+    v, p = page * d // 2, page * d // 64 * 4
+    cut = [0, v, 2 * v, 2 * v + p, 2 * v + 2 * p]
+    a = [pool[..., i:j].reshape(*pool.shape[:2], page, -1) for i, j in zip(cut, cut[1:])]
+    return [a[0], a[1]] + [np.ascontiguousarray(x).view(np.uint16).reshape(*x.shape[:3], d // 64, 2) for x in a[2:]]
+
+
+def held(pool, page, d):
+    """The values a pool stands for, f64 K and V [pages][heads][P][D] (CUDA)."""
+    kb, vb, kp, vp = parts(pool.cpu().numpy(), page, d)
+    got = []
+    for b, p in ((kb, kp), (vb, vp)):
+        n = np.stack([b & 15, b >> 4], -1).reshape(*b.shape[:3], d // 64, 64).astype(np.float64)
+        s = torch.from_numpy(p.astype(np.int32) << 16).view(torch.float32).double().numpy()
+        with np.errstate(invalid="ignore"):
+            got.append(torch.from_numpy((s[..., 1:] + s[..., :1] * n).reshape(*b.shape[:3], d)).to(DEV))
+    return got
+
+
+def f32_rotate(x, tab, pos, rot, inter):
+    cs = tab[pos.long()][:, None]
+    c, s = cs[..., 0], cs[..., 1]
+    y = x.float().clone()
+    i = torch.arange(rot // 2, device=DEV)
+    a, b = (2 * i, 2 * i + 1) if inter else (i, i + rot // 2)
+    xa, xb = x.float()[..., a], x.float()[..., b]
+    y[..., a], y[..., b] = xa * c - xb * s, xb * c + xa * s
+    return y
+
+
+def check_append(eng, d, page, rot, inter, tokens, hkv, hq, k, v, q, seed=0):
+    g = gen(seed + 50)
+    pages = 2 * tokens // page + 3
+    pool = torch.randint(0, 256, (pages, hkv, sage.Kv4Cache.block_bytes(d, page)), generator=g, device=DEV,
+                         dtype=torch.int32).to(torch.uint8)
+    before = pool.cpu().numpy().copy()
+    slots = torch.randperm(pages * page, generator=g, device=DEV)[:tokens].int()
+    if tokens > 2:
+        slots[1] = -1
+    tab = table(rot, 5000) if rot else None
+    pos = torch.randint(0, 5000, (tokens,), generator=g, device=DEV, dtype=torch.int32) if rot else None
+    cache = sage.Kv4Cache(pool, page, d)
+    more = {}
+    if rot:
+        more = dict(rotary=sage.Rotary(tab, rot, inter), positions=pos)
+    if hq:
+        q_out = torch.zeros(tokens, hq, d, dtype=torch.bfloat16, device=DEV)
+        more.update(q=q, q_out=q_out)
+    eng.kv4_append(cache, k, v, slots, **more)
+    kr = f32_rotate(k, tab, pos, rot, inter) if rot else k.float()
+    want = before.copy()
+    block = [quantise(x.float().cpu().numpy()) for x in (kr, v)]
+    half, par, ng = page * d // 2, page * d // 64 * 4, d // 64
+    for t, slot in enumerate(slots.tolist()):
+        if slot < 0:
+            continue
+        p, r = divmod(slot, page)
+        for i, (n, scale, zero) in enumerate(block):
+            byte = n[t, :, 0::2] | (n[t, :, 1::2] << 4)
+            want[p, :, i * half + r * d // 2:i * half + (r + 1) * d // 2] = byte
+            bits = torch.from_numpy(np.stack([scale[t], zero[t]], -1)).bfloat16().view(torch.int16).numpy()
+            at = 2 * half + i * par + r * ng * 4
+            want[p, :, at:at + ng * 4] = bits.reshape(hkv, -1).view(np.uint8)
+    got = pool.cpu().numpy()
+    a, b = parts(got, page, d), parts(want, page, d)
+    for i in (0, 1):
+        assert np.array_equal(a[i], b[i]), ("K values", "V values")[i]
+    for i in (2, 3):  # parameters as numbers: any NaN, either zero
+        x, y = (torch.from_numpy(w[i].astype(np.int32) << 16).view(torch.float32) for w in (a, b))
+        assert torch.equal(torch.nan_to_num(x, nan=123.5), torch.nan_to_num(y, nan=123.5)), ("K params", "V params")[i - 2]
+    if hq:
+        assert torch.equal(q_out, f32_rotate(q, tab, pos, rot, inter).bfloat16())
+    ko, vo = (torch.full((tokens, hkv, d), 5.0, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    eng.kv4_read(cache, slots, ko, vo)
+    kh, vh = held(pool, page, d)
+    p, r = (slots.clamp(min=0) // page).long(), (slots.clamp(min=0) % page).long()
+    for o, h in ((ko, kh), (vo, vh)):
+        w = h[p, :, r].float().bfloat16()  # scale * n is exact, the sum rounds once to f32, then to bf16
+        w[slots < 0] = 0
+        assert torch.equal(torch.nan_to_num(o, nan=99.0), torch.nan_to_num(w, nan=99.0))
+    eng.engine_status()
+    return pool
+
+
+@pytest.mark.parametrize("d,page,rot,inter", [(128, 64, 128, False), (64, 16, 64, False), (128, 16, 64, True),
+                                              (64, 128, 16, True), (128, 32, 96, False), (64, 32, 0, False),
+                                              (128, 128, 48, True)])
+@pytest.mark.parametrize("tokens,hkv,hq", [(1, 1, 0), (5, 2, 6), (130, 3, 7), (700, 8, 32)])
+def test_append_and_read(engines, d, page, rot, inter, tokens, hkv, hq):
+    if not rot:
+        hq = 0
+    g = gen(tokens + d)
+    qkv = rand(g, tokens, hq + 2 * hkv, d)
+    check_append(engines[d], d, page, rot, inter, tokens, hkv, hq, qkv[:, hq:hq + hkv], qkv[:, hq + hkv:], qkv[:, :hq])
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_append_of_uncommon_values(engines, d):
+    """Constant groups, ties, tiny and huge ranges, NaN and infinities, each in a group of its own."""
+    g, tokens = gen(9), 12
+    k, v = rand(g, tokens, 2, d).float(), rand(g, tokens, 2, d).float()
+    k[0] = 0.0
+    k[1] = -3.25
+    k[2, :, :64] = torch.arange(64, device=DEV) % 16          # exactly on the steps
+    k[3, :, :64] = (torch.arange(64, device=DEV) % 31) / 2    # ties between two of them
+    k[4] *= 2.0 ** -110
+    k[5] *= 2.0 ** 125
+    k[6, 0, 3], k[6, 1, d - 1] = math.nan, math.inf
+    k[7, 0, 0], k[7, 1, 63] = -math.inf, math.nan
+    v[0, 0, 0], v[1, 1, d - 1], v[2] = math.nan, -math.inf, 1.0
+    v[3, :, 0], v[3, :, 1] = 3.38e38, -3.38e38                # a range beyond f32
+    v[4] *= 1e-39                                             # subnormal
+    k, v = k.bfloat16(), v.bfloat16()
+    check_append(engines[d], d, 16, 0, False, tokens, 2, 0, k, v, None)
+    check_append(engines[d], d, 16, 32, True, tokens, 2, 0, k, v, None)
+
+
+def test_append_bad_slots_and_positions(engines):
+    eng, g, d, page = engines[128], gen(11), 128, 16
+    pool = torch.full((3, 2, sage.Kv4Cache.block_bytes(d, page)), 0xAB, dtype=torch.uint8, device=DEV)
+    before = pool.clone()
+    k, v, q = rand(g, 4, 2, d), rand(g, 4, 2, d), rand(g, 4, 4, d)
+    out = torch.full_like(q, 2.0)
+    r = sage.Rotary(table(128, 8), 128)
+    eng.kv4_append(sage.Kv4Cache(pool, page, d), k, v, ints([48, 2**31 - 1, 5, -1]), rotary=r,
+                   positions=ints([0, 1, 8, -1]), q=q, q_out=out)
+    assert torch.equal(pool, before) and (out == 2.0).all()
+    with pytest.raises(sage.SageError):
+        eng.engine_status()
+    ko, vo = torch.full_like(k, 4.0), torch.full_like(v, 4.0)
+    eng.kv4_read(sage.Kv4Cache(pool, page, d), ints([48, 47, -5, 2**31 - 1]), ko, vo)
+    assert (ko[[0, 3]] == 4.0).all() and (ko[2] == 0).all()
+    with pytest.raises(sage.SageError):
+        eng.engine_status()
+    eng.engine_status()
+
+
+def test_pool_of_strided_pages(engines):
+    """A pool that is every second page of a larger buffer, its heads cut from more."""
+    eng, g, d, page = engines[64], gen(12), 64, 32
+    block = sage.Kv4Cache.block_bytes(d, page)
+    big = torch.full((8, 5, block), 0x5A, dtype=torch.uint8, device=DEV)
+    pool = big[::2, 1:3]
+    k, v = rand(g, 6, 2, d), rand(g, 6, 2, d)
+    slots = ints([0, 31, 32, 127, 70, 64])
+    eng.kv4_append(sage.Kv4Cache(pool, page, d), k, v, slots)
+    dense = torch.full((4, 2, block), 0x5A, dtype=torch.uint8, device=DEV)
+    eng.kv4_append(sage.Kv4Cache(dense, page, d), k, v, slots)
+    assert torch.equal(pool, dense)
+    assert (big[1::2] == 0x5A).all() and (big[:, 0] == 0x5A).all() and (big[:, 3:] == 0x5A).all()
+
+
+# ---------------------------------------------------------------- attention
+
+class Batch:
+    """A cache filled with `kv` tokens a sequence, pages in a shuffled order,
+    ids behind the last needed page wild, and everything behind the last token
+    NaN; qn query tokens a sequence."""
+
+    def __init__(self, d, page, hq, hkv, kv, qn, seed=0, kscale=1.0, tail_rows=2):
+        g = gen(seed)
+        self.d, self.page, self.hq, self.hkv, self.kv, self.qn = d, page, hq, hkv, kv, qn
+        need = [-(-n // page) for n in kv]
+        pages = sum(need) + 2
+        block = sage.Kv4Cache.block_bytes(d, page)
+        self.pool = torch.full((pages, hkv, block), 0xFF, dtype=torch.uint8, device=DEV)  # bf16 0xffff: NaN
+        order = torch.randperm(pages, generator=g, device=DEV).cpu()
+        most = max(max(need), 1) + 1
+        ids = torch.full((len(kv), most), -7, dtype=torch.int32)
+        ids[:, -1] = 2**31 - 1
+        at, slots = 0, []
+        for i, n in enumerate(need):
+            ids[i, :n] = order[at:at + n]
+            j = torch.arange(kv[i])
+            slots.append(ids[i].long()[j // page] * page + j % page)
+            at += n
+        self.pages = ids.to(DEV)
+        self.slots = torch.cat(slots).int().to(DEV)
+        total = sum(kv)
+        offset = torch.randn(hkv, d, generator=g, device=DEV)
+        k = (torch.randn(total, hkv, d, generator=g, device=DEV) * kscale + offset).bfloat16()
+        v = rand(g, total, hkv, d)
+        self.eng = None
+        self.k, self.v = k, v
+        self.kv_len = ints(kv)
+        starts = np.concatenate([[0], np.cumsum(qn)])
+        self.q_start = ints(starts)
+        self.q = rand(g, int(starts[-1]) + tail_rows, hq, d)
+        self.out = torch.full_like(self.q, 3.0)
+        self.lse = torch.full((self.q.shape[0], hq), 5.0, device=DEV)
+
+    def fill(self, eng):
+        if self.slots.numel():
+            eng.kv4_append(sage.Kv4Cache(self.pool, self.page, self.d), self.k, self.v, self.slots)
+
+    def attend(self, eng, ws, **k):
+        a = dict(q_start=self.q_start, max_q=max(max(self.qn), 1), lse=self.lse)
+        a.update(k)
+        eng.kv4_attend(ws, sage.Kv4Cache(self.pool, self.page, self.d), self.q, self.out, self.pages, self.kv_len, **a)
+
+    def check(self, causal=True, window=0, scale=None, what=""):
+        d, hq, hkv, g = self.d, self.hq, self.hkv, self.hq // self.hkv
+        scale = d ** -0.5 if scale is None else scale
+        kb, vb, kp, vp = parts(self.pool.cpu().numpy(), self.page, d)
+        kh, vh = held(self.pool, self.page, d)
+        vs = torch.from_numpy(vp.astype(np.int32)[..., 0] << 16).view(torch.float32).double().to(DEV)
+        vn = torch.from_numpy(np.stack([vb & 15, vb >> 4], -1).reshape(*vb.shape[:3], d)).to(DEV).double()
+        row = 0
+        for b, (n, qn) in enumerate(zip(self.kv, self.qn)):
+            if qn == 0:
+                continue
+            p = self.pages[b, :-(-n // self.page)].long()
+            k, v = (x[p].transpose(1, 2).reshape(-1, hkv, d)[:n] for x in (kh, vh))
+            # a probability times its V scale is rounded to bf16, by at most 2^-8; it weighs n - 8
+            w = (vn[p].transpose(1, 2).reshape(-1, hkv, d)[:n] - 8).abs() * vs[p].transpose(1, 2).reshape(
+                -1, hkv, d // 64)[:n].repeat_interleave(64, -1)
+            j = torch.arange(n, device=DEV)
+            at = n - qn + torch.arange(qn, device=DEV)[:, None]
+            see = torch.ones(qn, n, dtype=torch.bool, device=DEV)
+            if causal:
+                see &= j <= at
+            if window:
+                see &= j > at - window
+            for h in range(hkv):
+                q = self.q[row:row + qn, h * g:(h + 1) * g].double()
+                x = torch.einsum("tgd,kd->tgk", q, k[:, h]) * scale
+                # f32 sums of scores: 24 roundings (products' sums of 4 steps per group, parameters) of the terms' size
+                most = 4 * w[:, h].amax() + 2 * k[:, h].abs().amax() if n else 0.0
+                size = q.abs().sum(-1) * most * scale
+                x = torch.where(see[:, None], x, -math.inf)
+                lse = torch.logsumexp(x, -1) if n else torch.full((qn, g), -math.inf, dtype=torch.float64, device=DEV)
+                pr = torch.where(see[:, None], torch.exp(x - torch.where(lse == -math.inf, 0.0, lse)[..., None]), 0.0)
+                o = torch.einsum("tgk,kd->tgd", pr, v[:, h])
+                off = 24 * 2.0 ** -24 * size + 2.0 ** -20
+                tol = (2.0 ** -8 * o.abs() + 2.0 ** -8 * torch.einsum("tgk,kd->tgd", pr, w[:, h])
+                       + (2 * off[..., None]) * (v[:, h].abs().amax() if n else 0.0) + 1e-30)
+                got = self.out[row:row + qn, h * g:(h + 1) * g].double()
+                bad = (got - o).abs() > tol
+                assert not bad.any(), (what, b, h, bad.nonzero()[:4].tolist(), (got - o).abs().max().item())
+                assert torch.isfinite(got).all()
+                if self.lse is not None:
+                    gl = self.lse[row:row + qn, h * g:(h + 1) * g].double()
+                    same = (gl == lse) | ((gl - lse).abs() <= off + 2.0 ** -22 * lse.abs())
+                    assert same.all(), (what, b, h, (gl - lse).abs().max().item())
+            row += qn
+        assert (self.out[row:] == 3.0).all() and (self.lse[row:] == 5.0).all()  # rows behind the last sequence
+
+
+HEADS = [(8, 2), (4, 4), (7, 1), (32, 8), (12, 1), (24, 1), (3, 1)]
+
+
+@pytest.mark.parametrize("d,page", [(64, 16), (64, 128), (128, 16), (128, 32), (128, 64)])
+@pytest.mark.parametrize("hq,hkv", HEADS)
+def test_attend_single_tokens(engines, d, page, hq, hkv):
+    """Decoding steps over every kind of length, an idle sequence among them."""
+    kv = [1, 2, 15, 16, 17, 31, 33, 0, 63, 64, 65, 127, 128, 129, 500, 1000, 3001]
+    b = Batch(d, page, hq, hkv, kv, [1] * len(kv), seed=d + page + hq)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    b.check(what="ragged")
+    b.attend(engines[d], engines["ws", d], causal=False, window=40)
+    b.check(causal=False, window=40, what="window")
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d,page,hq,hkv", [(128, 64, 32, 8), (64, 16, 6, 2), (128, 16, 7, 1), (128, 128, 4, 4),
+                                           (64, 64, 40, 1)])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 0), (True, 1), (True, 37), (False, 130), (True, 10000)])
+def test_attend_several_tokens(engines, d, page, hq, hkv, causal, window):
+    """Drafted tokens and pieces of prompts: more queries than keys (rows that
+    see nothing), sequences without queries, lengths of one."""
+    kv, qn = [5, 300, 1, 0, 77, 129, 640, 16], [5, 3, 1, 2, 0, 129, 200, 40]
+    b = Batch(d, page, hq, hkv, kv, qn, seed=hq + page)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], causal=causal, window=window)
+    b.check(causal, window)
+    small = Batch(d, page, hq, hkv, [4, 260, 1, 0, 33], [2, 2, 1, 2, 0], seed=hq + page + 1)
+    small.fill(engines[d])
+    small.attend(engines[d], engines["ws", d], causal=causal, window=window)
+    small.check(causal, window, what="two tokens")
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_one_long_sequence(engines, d):
+    """Split over the whole GPU; a softmax scale of its own, large scores."""
+    b = Batch(d, 64, 8, 2, [20011], [1], seed=3, kscale=3.0)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], softmax_scale=0.5)
+    b.check(scale=0.5)
+    b.attend(engines[d], engines["ws", d], softmax_scale=1e-4)
+    b.check(scale=1e-4)
+
+
+@pytest.mark.parametrize("d,hq,hkv", [(128, 8, 2), (64, 4, 4)])
+def test_attend_without_q_start(engines, d, hq, hkv):
+    kv = [3, 90, 17, 0]
+    b = Batch(d, 32, hq, hkv, kv, [1] * 4)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], q_start=None)
+    b.check()
+
+
+def test_attend_many_sequences(engines):
+    """More sequences than a warp has lanes, more tiles than CTAs."""
+    kv = [(i * 37) % 150 for i in range(300)]
+    b = Batch(64, 16, 8, 4, kv, [1] * 300)
+    b.fill(engines[64])
+    b.attend(engines[64], engines["ws", 64])
+    b.check()
+
+
+def test_attend_strided_rows(engines):
+    """q cut from a packed projection, out head-major."""
+    d, eng = 128, engines[128]
+    b = Batch(d, 64, 4, 2, [70, 9], [3, 2], tail_rows=0)
+    b.fill(eng)
+    wide = torch.zeros(5, 9, d, dtype=torch.bfloat16, device=DEV)
+    wide[:, 3:7] = b.q
+    b.q = wide[:, 3:7]
+    b.out = torch.full((4, 5, d), 3.0, dtype=torch.bfloat16, device=DEV).transpose(0, 1)
+    b.attend(eng, engines["ws", d])
+    b.check()
+
+
+@pytest.mark.parametrize("rows", [1, 4, 40])
+def test_attend_nan_reaches_only_the_rows_that_see_it(engines, rows):
+    """A cached NaN (K of one token, V of one group of another) spreads to
+    the queries that see it and to no other; a V group's only to its channels."""
+    d, eng, n = 128, engines[128], 100
+    for part in ("k", "v"):
+        b = Batch(d, 16, 2, 1, [n], [rows], tail_rows=0)
+        at = n - rows + rows // 2  # seen by the later half of the queries
+        getattr(b, part)[at, 0, 70] = math.nan
+        b.fill(eng)
+        b.attend(eng, engines["ws", d])
+        see = torch.arange(n - rows, n, device=DEV) >= at
+        nan = torch.isnan(b.out)
+        if part == "k":
+            assert nan[see].all() and not nan[~see].any()
+        else:
+            assert nan[see][..., 64:].all() and not nan[see][..., :64].any() and not nan[~see].any()
+    eng.engine_status()
+
+
+def test_attend_bad_indices_are_reported(engines):
+    """Wild page ids, lengths and q_start stay inside the buffers, set the
+    error word, and leave the other sequences right."""
+    d, eng, ws = 64, engines[64], engines["ws", 64]
+    b = Batch(d, 16, 2, 2, [40, 50, 60], [1, 1, 1], tail_rows=0)
+    b.fill(eng)
+    good = b.pages.clone()
+
+    def run(**k):
+        b.out.fill_(3.0)
+        b.attend(eng, ws, **k)
+        with pytest.raises(sage.SageError):
+            eng.engine_status()
+        return b.out.clone()
+
+    b.attend(eng, ws)
+    right = b.out.clone()
+    eng.engine_status()
+    b.pages[1, 1] = b.pool.shape[0]
+    assert torch.equal(run()[[0, 2]], right[[0, 2]])
+    b.pages[1, 1] = -1
+    assert torch.equal(run()[[0, 2]], right[[0, 2]])
+    b.pages.copy_(good)
+    b.kv_len[0] = -3
+    assert torch.equal(run()[1:], right[1:])
+    b.kv_len[0] = 40
+    b.q_start.copy_(ints([0, 1, 2, 9]))
+    assert torch.equal(run()[:2], right[:2])
+    b.q_start.copy_(ints([-5, 1, 2, 3]))
+    assert torch.equal(run()[1:], right[1:])
+    b.q_start.copy_(ints([0, 1, 2, 3]))
+    b.attend(eng, ws)
+    assert torch.equal(b.out, right)
+    eng.engine_status()
+
+
+def test_attend_is_reproducible_and_splits_do_not_matter_much(engines):
+    d, eng, ws = 128, engines[128], engines["ws", 128]
+    b = Batch(d, 64, 8, 2, [5000, 40, 9000], [1, 1, 1])
+    b.fill(eng)
+    b.attend(eng, ws)
+    first = b.out.clone()
+    for _ in range(5):
+        b.attend(eng, ws)
+        assert torch.equal(b.out, first)
+    eng.reserve_sms(100)
+    try:
+        b.attend(eng, ws)
+        b.check(what="fewer SMs")
+    finally:
+        eng.reserve_sms(0)
+
+
+# ---------------------------------------------------------------- as they are used
+
+@pytest.mark.parametrize("d,inter", [(128, False), (64, True)])
+def test_decoding_loop(engines, d, inter):
+    """A prompt laid down in two pieces, then tokens one by one: each step
+    rotates and appends, then attends; checked against the held values."""
+    eng, ws = engines[d], engines["ws", d]
+    hq, hkv, page, n, rot = 8, 2, 16, 90, d // 2
+    g = gen(21)
+    pool = torch.zeros(12, hkv, sage.Kv4Cache.block_bytes(d, page), dtype=torch.uint8, device=DEV)
+    cache = sage.Kv4Cache(pool, page, d)
+    pages = torch.randperm(12, generator=g, device=DEV).int()[None, :8].contiguous()
+    r = sage.Rotary(table(rot, 200), rot, inter)
+    x = rand(g, n, hq + 2 * hkv, d)
+    got = torch.zeros(n, hq, d, dtype=torch.bfloat16, device=DEV)
+    rotated = torch.zeros(n, hq, d, dtype=torch.bfloat16, device=DEV)
+    at = 0
+    for step in [50, 30] + [1] * 10:
+        sl = slice(at, at + step)
+        pos = torch.arange(at, at + step, device=DEV, dtype=torch.int32)
+        slots = (pages[0].long()[pos.long() // page] * page + pos.long() % page).int()
+        eng.kv4_append(cache, x[sl, hq:hq + hkv], x[sl, hq + hkv:], slots, rotary=r, positions=pos, q=x[sl, :hq],
+                       q_out=rotated[sl])
+        at += step
+        eng.kv4_attend(ws, cache, rotated[sl], got[sl], pages, ints([at]), q_start=ints([0, step]), max_q=step)
+    eng.engine_status()
+    b = Batch(d, page, hq, hkv, [n], [n], tail_rows=0)
+    b.pool, b.pages, b.q, b.out, b.lse = pool, pages, rotated, got, torch.zeros(n, hq, device=DEV)
+    check_lse = b.lse
+    b.lse = torch.zeros(n, hq, device=DEV)
+    eng.kv4_attend(ws, cache, rotated, torch.zeros_like(got), pages, ints([n]), q_start=ints([0, n]), max_q=n, lse=b.lse)
+    b.check()
+    del check_lse
+
+
+def test_read_gives_a_prefix_to_the_dense_kernel(engines):
+    """The values read back are what attention over the cache sees: the
+    dense kernel on them agrees within its own quantisation."""
+    d, eng, n = 128, engines[128], 256
+    b = Batch(d, 64, 4, 4, [n], [n], tail_rows=0)
+    b.fill(eng)
+    b.attend(eng, engines["ws", d])
+    k, v = (torch.empty(n, 4, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    eng.kv4_read(sage.Kv4Cache(b.pool, 64, d), b.slots, k, v)
+    w = eng.workspace(sage.Shape(1, 4, n, causal=True))
+    o = torch.empty_like(k)
+    st = sage.Strides.bthd(n, 4, d)
+    eng.forward(w, *[sage.Tensor(t, st) for t in (b.q, k, v, o)])
+    e = (o.float() - b.out.float()).norm() / b.out.float().norm()
+    assert e < 0.04  # the reference's gate for its quantised attention (rel-L2)
+
+
+def test_graph_replays_match_eager_calls(engines):
+    """Append and attend captured once, replayed on new inputs, lengths and slots."""
+    d, page, hq, hkv, nb = 128, 16, 8, 2, 3
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        eng = sage.SageAttention(s, d)
+        ws = eng.kv4_workspace()
+        pool = torch.zeros(20, hkv, sage.Kv4Cache.block_bytes(d, page), dtype=torch.uint8, device=DEV)
+        twin = pool.clone()
+        pages = torch.arange(18, device=DEV, dtype=torch.int32).view(nb, 6).contiguous()
+        x = torch.zeros(nb, hq + 2 * hkv, d, dtype=torch.bfloat16, device=DEV)
+        pos, kv, slots = (torch.zeros(nb, dtype=torch.int32, device=DEV) for _ in range(3))
+        q, out = (torch.zeros(nb, hq, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+        r = sage.Rotary(table(d, 128), d)
+
+        def step(p):
+            c = sage.Kv4Cache(p, page, d)
+            eng.kv4_append(c, x[:, hq:hq + hkv], x[:, hq + hkv:], slots, rotary=r, positions=pos, q=x[:, :hq], q_out=q)
+            eng.kv4_attend(ws, c, q, out, pages, kv)
+
+        step(pool)
+        s.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph, stream=s):
+            step(pool)
+        pool.zero_()
+        twin.zero_()
+        g = gen(5)
+        for t in range(70):
+            x.copy_(rand(g, nb, hq + 2 * hkv, d))
+            n = torch.tensor([t, max(0, t - 20), t // 2], device=DEV)
+            pos.copy_(n)
+            kv.copy_(n + 1)
+            slots.copy_((pages.long()[torch.arange(nb, device=DEV), n // page] * page + n % page))
+            graph.replay()
+            a = out.clone()
+            step(twin)
+            assert torch.equal(a, out) and torch.equal(pool, twin), t
+        eng.engine_status()
+    s.synchronize()
+    del graph
+
+
+def test_two_streams_with_workspaces_of_their_own(engines):
+    """Calls in flight at once on two streams, an engine and workspace each."""
+    d = 128
+    sets = []
+    for i in range(2):
+        s = torch.cuda.Stream()
+        with torch.cuda.stream(s):
+            eng = sage.SageAttention(s, d)
+            ws = eng.kv4_workspace()
+            b = Batch(d, 64, 8, 2, [7000 + 999 * i, 30], [1, 1], seed=30 + i)
+            b.fill(eng)
+        s.synchronize()
+        sets.append((s, eng, ws, b))
+    torch.cuda.synchronize()
+    for _ in range(20):
+        for s, eng, ws, b in sets:
+            b.attend(eng, ws)
+    torch.cuda.synchronize()
+    for s, eng, ws, b in sets:
+        b.check()
+        eng.engine_status()
+
+
+def test_long_cache_passes_32_bit_offsets(engines):
+    """Slots and pages whose byte offsets pass 2^32: the pool is 6 GB, its last
+    pages are used."""
+    d, page, hkv = 128, 128, 8
+    eng, ws = engines[d], engines["ws", d]
+    block = sage.Kv4Cache.block_bytes(d, page)
+    pages = 6 * 10**9 // (block * hkv)
+    pool = torch.empty(pages, hkv, block, dtype=torch.uint8, device=DEV)
+    g = gen(8)
+    n = 300
+    ids = ints([[pages - 1, pages - 2, pages // 2 + 1]])
+    k, v, q = rand(g, n, hkv, d), rand(g, n, hkv, d), rand(g, 1, 16, d)
+    j = torch.arange(n, device=DEV)
+    slots = (ids[0].long()[j // page] * page + j % page).int()
+    cache = sage.Kv4Cache(pool, page, d)
+    eng.kv4_append(cache, k, v, slots)
+    ko, vo, out = torch.empty_like(k), torch.empty_like(v), torch.empty_like(q)
+    eng.kv4_read(cache, slots, ko, vo)
+    small = torch.empty(3, hkv, block, dtype=torch.uint8, device=DEV)
+    c2 = sage.Kv4Cache(small, page, d)
+    eng.kv4_append(c2, k, v, j.int())
+    k2, v2, o2 = torch.empty_like(k), torch.empty_like(v), torch.empty_like(q)
+    eng.kv4_read(c2, j.int(), k2, v2)
+    eng.kv4_attend(ws, cache, q, out, ids, ints([n]))
+    eng.kv4_attend(ws, c2, q, o2, ints([[0, 1, 2]]), ints([n]))
+    assert torch.equal(ko, k2) and torch.equal(vo, v2) and torch.equal(out, o2)
+    assert torch.equal(pool[ids[0].long()[0]], small[0])
+    eng.engine_status()
+
+
+def test_gpu_refusals(engines):
+    """What the wrappers refuse: types, shapes, devices, mixed-up arguments."""
+    d, eng, ws = 128, engines[128], engines["ws", 128]
+    g = gen(1)
+    x = rand(g, 4, 2, d)
+    r = sage.Rotary(table(64, 10), 64)
+    pos = ints([0, 1, 2, 3])
+    cache = sage.Kv4Cache.empty(4, 2, 16, d)
+    with pytest.raises(sage.SageError):
+        eng.rope(x, x.float(), r, pos)
+    with pytest.raises(sage.SageError):
+        eng.rope(x, torch.empty_like(x), r, pos.long())
+    with pytest.raises(sage.SageError):
+        eng.rope(x, torch.empty_like(x), r, pos[:3])
+    with pytest.raises(sage.SageError):
+        eng.rope(x.cpu(), torch.empty_like(x), r, pos)
+    with pytest.raises(sage.SageError):
+        eng.rope(x[..., :64], torch.empty_like(x[..., :64]), r, pos)
+    with pytest.raises(sage.SageError):
+        engines[64].kv4_append(cache, x, x, pos)
+    with pytest.raises(sage.SageError):
+        eng.kv4_append(cache, x, x, pos, rotary=r)
+    with pytest.raises(sage.SageError):
+        eng.kv4_append(cache, x.half(), x, pos)
+    with pytest.raises(sage.SageError):
+        eng.kv4_append(cache, x, x, pos, q=x)
+    with pytest.raises(sage.SageError):
+        eng.kv4_read(cache, pos, x[:, :1], x)
+    q, o, kv, ids = rand(g, 4, 4, d), rand(g, 4, 4, d), ints([1] * 4), ints([[0]] * 4)
+    for bad in (dict(q_start=pos), dict(window=-1), dict(window=2**32), dict(max_q=2), dict(softmax_scale=-1.0),
+                dict(lse=torch.zeros(4, 4, device=DEV, dtype=torch.float64))):
+        with pytest.raises(sage.SageError):
+            eng.kv4_attend(ws, cache, q, o, ids, kv, **bad)
+    with pytest.raises(sage.SageError):
+        eng.kv4_attend(engines["ws", 64], cache, q, o, ids, kv)
+    with pytest.raises(sage.SageError):
+        eng.kv4_attend(ws, cache, rand(g, 4, 3, d), rand(g, 4, 3, d), ids, kv)
+    with pytest.raises(sage.SageError):
+        eng.kv4_attend(ws, cache, q, q, ids, kv)
+    with pytest.raises(sage.SageError):
+        sage.Kv4Cache(torch.zeros(4, 2, 100, dtype=torch.uint8, device=DEV), 16, d)
+    closed = eng.kv4_workspace()
+    closed.close()
+    with pytest.raises(sage.SageError):
+        eng.kv4_attend(closed, cache, q, o, ids, kv)
+    eng.engine_status()
