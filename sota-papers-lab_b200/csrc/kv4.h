@@ -63,15 +63,20 @@ struct Kv4Attend {
     const int* pages;    // [batch][max_pages]
     int max_pages;
     int batch, heads, group, tokens, max_q;  // group = heads / kv_heads
+    uint32_t group_mul;   // n / group = (n * group_mul) >> (32 + group_shift) for n < 2^31; 0: group is 1
+    int group_shift;
     int causal, window;
     float c;  // softmax scale * log2(e)
     void* scratch;        // kv4_scratch_bytes
+    uint32_t* done;       // (set by the launch) [CTAs] pieces of a split tile that are finished, zero between calls
     float2* part_ml;      // (set by the launch) [2 * CTAs][cols] running maximum (log2) and sum of split tiles
     float* part_o;        // (set by the launch) [2 * CTAs][cols][D] their outputs
     uint32_t* err;
 };
 
-// Scratch of one attend call: partial outputs of at most two pieces per CTA.
+// Scratch of one attend call: partial outputs of at most two pieces per CTA,
+// behind counts that must be zero before the first call.
+constexpr size_t KV4_COUNTS = 8192;  // bytes
 size_t kv4_scratch_bytes(int d, int sms);
 cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t st);
 

@@ -288,7 +288,9 @@ int spl_sage_kv4_ws_create(spl_sage* s, spl_sage_kv4_ws** out) {
     ws->device = s->device;
     ws->head_dim = s->head_dim;
     ws->bytes = sp::kv4_scratch_bytes(s->head_dim, s->sm_count);
-    const cudaError_t e = cudaMalloc(&ws->mem, ws->bytes);
+    cudaError_t e = cudaMalloc(&ws->mem, ws->bytes);
+    if (e == cudaSuccess && (e = cudaMemsetAsync(ws->mem, 0, sp::KV4_COUNTS, s->stream)) != cudaSuccess)
+        cudaFree(ws->mem);
     if (e != cudaSuccess) {
         delete ws;
         return cuda_fail(e, "allocate the cache attention's workspace");
@@ -360,6 +362,10 @@ int spl_sage_kv4_attend(spl_sage* s, spl_sage_kv4_ws* ws, const spl_sage_kv4* ca
     a.batch = (int)sh.batch;
     a.heads = (int)sh.heads;
     a.group = (int)(sh.heads / hk);
+    if (a.group > 1) {
+        while ((2 << a.group_shift) < a.group) a.group_shift++;
+        a.group_mul = (uint32_t)(((uint64_t)1 << (32 + a.group_shift)) / a.group + 1);
+    }
     a.tokens = (int)sh.tokens;
     a.max_q = (int)sh.max_q;
     a.causal = sh.causal ? 1 : 0;

@@ -19,20 +19,19 @@
 //   - K's scale and zero are per key and group of 64 channels: each group's
 //     sum is kept apart and S = s0 a0 + s1 a1 + (z0 Q0 + z1 Q1), Q the row's
 //     channel sums.  So S is that of the exact cached values, to f32.
-//   - V's n sits at mantissa bits 3-6 of a bf16 with exponent 2^4: 16 + n.  V's
-//     scale goes into the probability (one bf16 rounding of p * s, 2^-9
-//     relative; bf16 has the range of any scale), and o = sum(p s (n - 8)) +
-//     sum(p (z + 8 s)): 24 * sum(p s) is taken out of the first sum through
-//     one more product with ones (of the same rounded p s), the second is kept
-//     in f32.  About n's middle the rounding weighs |n - 8| instead of n: the
-//     output's error against 64 bits fell from 0.0038 to 0.0020 (0.0017 is
-//     the rounding of the output itself).
+//   - V's n enters the same way.  Its scale goes into the probability, in f16:
+//     p * s * 2^(14 - R), where 2^R bounds the scales the warp has met so far,
+//     is rounded once by 2^-12 of itself (2^-25 * 2^-14 of the largest where it
+//     is subnormal); R rises, and the sums are scaled, when a scale comes near
+//     the end of f16's range.  sum(p z) is kept in f32.
 //   - S^T has a key per row, P^T wants the keys along k: movmatrix transposes
 //     the 8x8 blocks in registers.
 // Each of the 8 warps streams its own 32-key steps through its own ring in
 // shared memory (cp.async, 16 bytes, no barrier but the warp's own) with its
 // own running maximum and sums; the warps meet once per tile.  Row maxima are
 // looked at by vote and only recomputed when one grows.
+#include <atomic>
+
 #include "kv4_sched.cuh"
 #include "sage_kernels.h"
 
@@ -49,8 +48,12 @@ struct AttnCfg {
     static constexpr int STAGE = 2 * VAL + 2 * PAR;        // D = 128: 4608, D = 64: 2304
     static constexpr int STAGES = D == 128 ? 3 : 4;
     static constexpr int COLS = 8 * NT;
-    static constexpr int WARP = STAGE * STAGES;            // ring of a warp, and its output at a tile's end
-    static_assert(WARP >= COLS * D * 4, "the ring holds a warp's output");
+    // A warp's memory: its ring, and its output at a tile's end.  The output
+    // takes the ring's last stage where it fits (the next tile's first steps
+    // are loaded into the others meanwhile).
+    static constexpr bool OVER = STAGE >= COLS * D * 4;
+    static constexpr int OUT = OVER ? STAGE * (STAGES - 1) : STAGE * STAGES;
+    static constexpr int WARP = OVER ? STAGE * STAGES : STAGE * STAGES + COLS * D * 4;
     static constexpr int SMEM = AT_WARPS * WARP;
 };
 
@@ -59,10 +62,17 @@ __device__ __forceinline__ void mma_f16(float (&d)[4], const uint32_t (&a)[4], u
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
-        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+__device__ __forceinline__ uint32_t pack_f16x2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+__device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
+// The same from zero.
+__device__ __forceinline__ void mma_f16_0(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%10,%10,%10,%10};"
+        : "=f"(d[0]), "=f"(d[1]), "=f"(d[2]), "=f"(d[3])
+        : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1), "f"(0.f));
 }
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
     uint32_t y;
@@ -102,34 +112,70 @@ __device__ __forceinline__ int stage_at(int key, int byte) {
 }
 
 // One lane's part of the copy of a 32-key step: `id0`, `id1` the pages of its
-// two halves of 16 keys (-1: none, zeros), key0 the step's first key.
+// two halves of 16 keys (-1: none, zeros), key0 the step's first key.  Every
+// source is a base of the half plus a constant.
 template <int D, int NT>
-__device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, long long head_off, int key0, int id0,
+__device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, const uint8_t* head, int key0, int id0,
                                           int id1) {
     using C = AttnCfg<D, NT>;
-    const int lane = threadIdx.x & 31, P = a.pool.page_tokens, mask = P - 1;
-    const uint8_t* b0 = a.pool.data + (long long)max(id0, 0) * a.pool.page_stride + head_off;
-    const uint8_t* b1 = a.pool.data + (long long)max(id1, 0) * a.pool.page_stride + head_off;
+    constexpr int PIECES = C::VAL / 16 / 32;  // of K values a lane copies: 4 or 2, half of them in each half
+    constexpr int PP = C::PAR / 16;           // parameter pieces of K: 16 or 8
+    const int lane = threadIdx.x & 31, P = a.pool.page_tokens;
+    const int in0 = key0 & (P - 1), in1 = (key0 + 16) & (P - 1);
+    const uint8_t* b0 = head + (uint64_t)(uint32_t)max(id0, 0) * (uint64_t)a.pool.page_stride;
+    const uint8_t* b1 = head + (uint64_t)(uint32_t)max(id1, 0) * (uint64_t)a.pool.page_stride;
     const int half = P * C::ROW;
-    constexpr int PIECES = C::VAL / 16 / 32;  // of K values a lane copies: 4 or 2
+    const uint32_t dst = stage + stage_at<D>(lane / (C::ROW / 16), lane % (C::ROW / 16) * 16);
 #pragma unroll
-    for (int r = 0; r < PIECES; r++) {
-        const int p = lane + 32 * r, key = p / (C::ROW / 16), byte = p % (C::ROW / 16) * 16;
-        const bool first = r < PIECES / 2;
-        const uint8_t* src = (first ? b0 : b1) + ((key0 + key) & mask) * C::ROW + byte;
-        const bool real = (first ? id0 : id1) >= 0;
-        const uint32_t dst = stage + stage_at<D>(key, byte);
-        cp_async16(dst, src, real);
-        cp_async16(dst + C::VAL, src + half, real);
+    for (int h = 0; h < 2; h++) {
+        const uint8_t* k = (h ? b1 : b0) + (h ? in1 : in0) * C::ROW + lane * 16;
+        const uint8_t* v = k + half;
+        const bool real = (h ? id1 : id0) >= 0;
+#pragma unroll
+        for (int r = 0; r < PIECES / 2; r++) {
+            cp_async16(dst + h * (C::VAL / 2) + r * 512, k + r * 512, real);
+            cp_async16(dst + C::VAL + h * (C::VAL / 2) + r * 512, v + r * 512, real);
+        }
     }
-    constexpr int PP = C::PAR / 16;  // parameter pieces of K: 16 or 8
     if (lane < 2 * PP) {
-        const int p = lane % PP, key = p * (16 / (C::NG * 4));
-        const bool first = p < PP / 2;
-        const uint8_t* src = (first ? b0 : b1) + 2 * half + (lane >= PP ? P * C::NG * 4 : 0) +
-                             ((key0 + key) & mask) * (C::NG * 4);
-        cp_async16(stage + 2 * C::VAL + lane * 16, src, (first ? id0 : id1) >= 0);
+        const bool second = (lane % PP) >= PP / 2;
+        const uint8_t* src = (second ? b1 : b0) + 2 * half + (lane >= PP ? P * C::NG * 4 : 0) +
+                             (second ? in1 : in0) * (C::NG * 4) + lane % (PP / 2) * 16;
+        cp_async16(stage + 2 * C::VAL + lane * 16, src, (second ? id1 : id0) >= 0);
     }
+}
+
+// The part of a tile that a CTA works on: its units unit0 .. unit1 - 1.
+struct Piece {
+    Place at;
+    KeyRange kr;
+    int unit0, unit1;
+    bool any;  // there is such a piece
+};
+
+template <int COLS>
+__device__ __forceinline__ void cut_piece(const Kv4Attend& a, const Shares& sh, long long from, Piece& p) {
+    p.kr = keys_of<COLS, AT_UNIT>(a, p.at.s, p.at.tile);
+    p.unit0 = (int)(from - p.at.start);
+    p.unit1 = (int)min((long long)p.kr.units, sh.first(blockIdx.x + 1) - p.at.start);
+}
+
+// The piece after p in the CTA's share.
+template <int COLS>
+__device__ __forceinline__ void next_piece(const Kv4Attend& a, const Shares& sh, const Piece& p, Piece& n) {
+    n.any = p.at.start + p.unit1 < sh.first(blockIdx.x + 1);
+    if (!n.any) return;
+    n.at = p.at;
+    n.at.start += p.kr.units;
+    if (++n.at.tile >= n.at.s.tiles) {
+        n.at.tile = 0;
+        if (++n.at.head >= a.pool.kv_heads) {
+            n.at.head = 0;
+            do n.at.s = seq_at<COLS>(a, ++n.at.b);  // (units are left: there is one)
+            while (n.at.s.tiles == 0);
+        }
+    }
+    cut_piece<COLS>(a, sh, n.at.start, n);
 }
 
 // Four channels of row n of the sequence, from sums relative to 2^ref.  A row
@@ -137,7 +183,7 @@ __device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, lo
 template <int D>
 __device__ __forceinline__ void put_row(const Kv4Attend& a, const Seq& s, int kv_head, int n, int d, float4 v, float ref,
                                         float sum) {
-    const int tok = n / a.group, head = kv_head * a.group + n - tok * a.group;
+    const int tok = by_group(a, n), head = kv_head * a.group + n - tok * a.group;
     const float inv = 1.f / sum;
     uint2 r = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
     if (sum == 0.f) r = make_uint2(0u, 0u);
@@ -146,130 +192,240 @@ __device__ __forceinline__ void put_row(const Kv4Attend& a, const Seq& s, int kv
         a.lse[(long long)(s.row0 + tok) * a.heads + head] = (ref + log2f(sum)) * 0.6931471805599453f;
 }
 
+// Joins the pieces that CTAs c0 .. c1 left of a tile's `cols` columns from row
+// n0 on.  D/4 threads hold a column's channels; where columns are few, the
+// pieces of one are shared out among several such teams, which meet in `sm`
+// (each warp's output area, WARP bytes apart) and `sm_ml`.
+template <int D, int COLS, int WARP>
+__device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int head, int n0, int cols, int c0, int c1,
+                                          uint8_t* sm, float2* sm_ml) {
+    constexpr int LANES = D / 4, TEAMS = AT_WARPS * 32 / LANES;
+    const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+    int slices = 1;
+    while (2 * slices * cols <= TEAMS) slices *= 2;
+    const int per = TEAMS / slices, slice = team / per;  // columns at a time
+    auto sm_v = [&](int t) { return (float4*)(sm + t * LANES / 32 * WARP) + t * LANES % 32 + lane; };
+    for (int first = 0; first < cols; first += per) {
+        const int col = first + team % per;
+        float m = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        // a few pieces at a time, all of their loads under way before the first is used
+        constexpr int AHEAD = 8;
+        for (int b = c0 + slice; b <= c1; b += slices * AHEAD) {
+            float2 ml[AHEAD];
+            float4 y[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int c = b + i * slices;
+                ml[i] = make_float2(-INFINITY, 0.f);
+                y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c <= c1 && col < cols) {
+                    const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
+                    ml[i] = __ldcg(&a.part_ml[slot]);
+                    y[i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
+                }
+            }
+            const float old = m;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) m = fmaxf(m, ml[i].x);
+            const float ref = m == -INFINITY ? 0.f : m, f0 = ex2(old - ref);
+            sum *= f0;
+            v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const float f = ex2(ml[i].x - ref);
+                sum = fmaf(f, ml[i].y, sum);
+                v.x = fmaf(f, y[i].x, v.x); v.y = fmaf(f, y[i].y, v.y);
+                v.z = fmaf(f, y[i].z, v.z); v.w = fmaf(f, y[i].w, v.w);
+            }
+        }
+        *sm_v(team) = v;
+        if (lane == 0) sm_ml[team] = make_float2(m, sum);
+        __syncthreads();
+        if (slice == 0 && col < cols) {
+            float mm = -INFINITY;
+            for (int i = 0; i < slices; i++) mm = fmaxf(mm, sm_ml[team + i * per].x);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            sum = 0.f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < slices; i++) {
+                const float2 ml = sm_ml[team + i * per];
+                const float4 y = *sm_v(team + i * per);
+                const float f = ex2(ml.x - ref);
+                sum = fmaf(f, ml.y, sum);
+                v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
+                v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+            }
+            put_row<D>(a, s, head, n0 + col, 4 * lane, v, ref, sum);
+        }
+        __syncthreads();
+    }
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(const __grid_constant__ Kv4Attend a) {
     using C = AttnCfg<D, NT>;
     constexpr int NG = C::NG, COLS = C::COLS, MT = 4;  // MT: tiles of 16 channels of a group
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ float sm_m[AT_WARPS][COLS], sm_l[AT_WARPS][COLS];
+    __shared__ uint16_t sm_q[NT * NG * 4 * 32 * 4];     // q fragments [nt][group][j][lane][4]
+    __shared__ float sm_cf[COLS], sm_qs[NG][COLS];
+    __shared__ bool sm_last;
+    __shared__ float2 sm_join[AT_WARPS * 2];
+    __shared__ Shares sh;
+    // The piece at work, the next and (a slow warp may still look at it) the
+    // last: what changes between them stays out of registers.
+    __shared__ Piece pieces[3];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
     const uint32_t ring = smem_u32(smem) + warp * C::WARP;
-    float* const sm_o = (float*)(smem + warp * C::WARP);  // [COLS][D] at a tile's end
+    float* const sm_o = (float*)(smem + warp * C::WARP + C::OUT);
 
+    // The lane's places in a stage.  K: key (g >> 1) + 4 (g & 1) (+ 8 and + 16
+    // keep the swizzle), group gr; V: key c + 4 i, where an odd i or, at D =
+    // 128, the second group is the other half of the row (D = 64: two rows on).
+    uint32_t k_off[NG], v_off[2];
+#pragma unroll
+    for (int gr = 0; gr < NG; gr++) k_off[gr] = stage_at<D>((g >> 1) + 4 * (g & 1), gr * 32 + c * 8);
+    v_off[0] = C::VAL + stage_at<D>(c, g * 4);
+    v_off[1] = C::VAL + stage_at<D>(c + 4, g * 4) - 4 * C::ROW;
+    const uint32_t p_off = 2 * C::VAL + ((g >> 1) + 4 * (g & 1)) * (NG * 4);
+
+    griddep_wait();
     griddep_launch_dependents();
     if (blockIdx.x == 0)  // what is out of range is reported once
         for (int b = threadIdx.x; b < a.batch; b += blockDim.x) seq_at<COLS>(a, b, true);
-    long long total, none;
-    count_units<COLS, AT_UNIT>(a, 0, total, none);
-    total *= a.pool.kv_heads;
-    const int G = shares(total, gridDim.x);
-    if ((int)blockIdx.x >= G) return;
-    long long u = first_unit(blockIdx.x, total, G);
-    const long long u_end = first_unit(blockIdx.x + 1, total, G);
-    const long long u_begin = u;
-    Place at = find_unit<COLS, AT_UNIT>(a, u);
+    if (warp == 0) {
+        Shares share;
+        Piece p;
+        p.any = find_share<COLS, AT_UNIT>(a, blockIdx.x, gridDim.x, share, p.at);
+        if (p.any) cut_piece<COLS>(a, share, share.first(blockIdx.x), p);
+        if (lane == 0) {
+            sh = share;
+            pieces[0] = p;
+        }
+    }
+    __syncthreads();
+    if (!pieces[0].any) return;
 
-    while (u < u_end) {
-        const Seq s = seq_at<COLS>(a, at.b);
-        const KeyRange kr = keys_of<COLS, AT_UNIT>(a, s, at.tile);
-        const long long tile_end = at.start + kr.units, piece_end = min(tile_end, u_end);
-        const int k0 = kr.lo + (int)(u - at.start) * AT_UNIT;
-        const int k1 = min(kr.hi, kr.lo + (int)(piece_end - at.start) * AT_UNIT);
-        const int n0 = at.tile * COLS, rows = s.qn * a.group;
-        const long long head_off = (long long)at.head * a.pool.block;
-        const int* ids = a.pages + (long long)at.b * a.max_pages;
-
-        // ---- page ids of the warp's next 16 steps, one lane per 16 keys
-        const int steps = max(0, (k1 - k0 + AT_STEP - 1) / AT_STEP - warp + AT_WARPS - 1) / AT_WARPS;
-        auto fetch_ids = [&](int step0) {
-            const int key = k0 + ((step0 + (lane >> 1)) * AT_WARPS + warp) * AT_STEP + 16 * (lane & 1);
-            int id = -1;
-            if (key < k1 && key + 16 > kr.first) {
-                id = ids[key >> a.pool.page_shift];
-                if (id < 0 || id >= a.pool.pages) {
-                    atomicOr(a.err, ERR_INDEX);
-                    id = -1;
-                }
+    // A piece's keys [k0, k1): the warps take its 32-key steps in turn.
+    auto first_key = [&](const Piece& p) { return p.kr.lo + p.unit0 * AT_UNIT; };
+    auto end_key = [&](const Piece& p) { return min(p.kr.hi, p.kr.lo + p.unit1 * AT_UNIT); };
+    auto steps_of = [&](int k0, int k1) {
+        return max(0, (k1 - k0 + AT_STEP - 1) / AT_STEP - warp + AT_WARPS - 1) / AT_WARPS;
+    };
+    // The page ids of 16 of the warp's steps from step0 on, one lane per 16
+    // keys; -1 where no key is wanted.
+    auto fetch_ids = [&](const Piece& p, int step0) {
+        const int key = first_key(p) + ((step0 + (lane >> 1)) * AT_WARPS + warp) * AT_STEP + 16 * (lane & 1);
+        int id = -1;
+        if (key < end_key(p) && key + 16 > p.kr.first) {
+            id = a.pages[(long long)p.at.b * a.max_pages + (key >> a.pool.page_shift)];
+            if (id < 0 || id >= a.pool.pages) {
+                atomicOr(a.err, ERR_INDEX);
+                id = -1;
             }
-            return id;
-        };
-        int cur_ids = fetch_ids(0), next_ids = steps > 16 ? fetch_ids(16) : -1;
-        auto issue = [&](int i) {
-            if (i < steps) {
-                if (i && (i & 15) == 0) {
-                    cur_ids = next_ids;
-                    next_ids = i + 16 < steps ? fetch_ids(i + 16) : -1;
-                }
-                const int id0 = __shfl_sync(0xffffffffu, cur_ids, 2 * (i & 15));
-                const int id1 = __shfl_sync(0xffffffffu, cur_ids, 2 * (i & 15) + 1);
-                load_step<D, NT>(a, ring + (i % C::STAGES) * C::STAGE, head_off,
-                                 k0 + (i * AT_WARPS + warp) * AT_STEP, id0, id1);
+        }
+        return id;
+    };
+    int cur_ids = fetch_ids(pieces[0], 0), next_ids = -1;
+    int fill, stage;  // the ring's stage to fill next, and to use next
+    auto issue = [&](const Piece& p, int i, int steps) {
+        if (i < steps) {
+            if (i && (i & 15) == 0) {
+                cur_ids = next_ids;
+                next_ids = i + 16 < steps ? fetch_ids(p, i + 16) : -1;
             }
-            cp_commit();
-        };
+            const int id0 = __shfl_sync(0xffffffffu, cur_ids, 2 * (i & 15));
+            const int id1 = __shfl_sync(0xffffffffu, cur_ids, 2 * (i & 15) + 1);
+            load_step<D, NT>(a, ring + fill * C::STAGE, a.pool.data + (long long)p.at.head * a.pool.block,
+                             first_key(p) + (i * AT_WARPS + warp) * AT_STEP, id0, id1);
+        }
+        fill = fill + 1 == C::STAGES ? 0 : fill + 1;
+        cp_commit();
+    };
+    // The lane's channels of the query rows that the warp prepares.
+    uint2 q_raw[NT];
+    auto load_q = [&](const Piece& p) {
 #pragma unroll
-        for (int i = 0; i < C::STAGES - 1; i++) issue(i);
+        for (int nt = 0; nt < NT; nt++) {
+            const int n = p.at.tile * COLS + 8 * nt + warp;
+            q_raw[nt] = make_uint2(0u, 0u);
+            if (n < p.at.s.qn * a.group && lane < D / 4) {
+                const int tok = by_group(a, n);
+                q_raw[nt] = *(const uint2*)((const uint16_t*)a.q.data + (p.at.s.row0 + tok) * a.q.st +
+                                            (p.at.head * a.group + n - tok * a.group) * a.q.sh + 4 * lane);
+            }
+        }
+    };
+    auto begin = [&](const Piece& p) {
+        const int steps = steps_of(first_key(p), end_key(p));
+        fill = stage = 0;
+        next_ids = steps > 16 ? fetch_ids(p, 16) : -1;
+#pragma unroll
+        for (int i = 0; i < C::STAGES - 1; i++) issue(p, i, steps);
+        load_q(p);
+    };
+    begin(pieces[0]);
 
-        // ---- the query rows as B fragments: column g, channels in the order
-        // of K's nibbles; and per column pair the lane's constants
+    for (int turn = 0;; turn = turn == 2 ? 0 : turn + 1) {
+        const Piece& p = pieces[turn];
+        Piece& next = pieces[turn == 2 ? 0 : turn + 1];
+        const Seq s = p.at.s;
+        const int k0 = first_key(p), k1 = end_key(p), steps = steps_of(k0, k1);
+        const int n0 = p.at.tile * COLS, rows = s.qn * a.group;
+        if (threadIdx.x == blockDim.x - 1) next_piece<COLS>(a, sh, p, next);
+
+        // ---- the query rows as B fragments, column by column: channel 16c +
+        // 4i + j of a group is half-word i of lane c's fragment j, the order
+        // of K's nibbles.  A warp makes columns `warp` and, with NT = 2, 8 on.
+#pragma unroll
+        for (int nt = 0; nt < NT; nt++) {
+            const int col = 8 * nt + warp;
+            const uint2 w = q_raw[nt];
+            float x[4] = {bf_lo(w.x), bf_hi(w.x), bf_lo(w.y), bf_hi(w.y)};
+            const float lane_max = fmaxf(fmaxf(fabsf(x[0]), fabsf(x[1])), fmaxf(fabsf(x[2]), fabsf(x[3])));
+            const float amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(lane_max)));
+            // 2^k brings the row's largest magnitude to [2^13, 2^14)
+            const int e = (int)(__float_as_uint(amax) >> 23) - 127;
+            const int k = min(max(13 - e, -100), 100);
+            float sum = 0.f;
+            if (lane < D / 4) {
+                uint16_t* dst = sm_q + (((nt * NG + lane / 16) * 4) * 32 + warp * 4 + lane % 16 / 4) * 4 + lane % 4;
+#pragma unroll
+                for (int j = 0; j < 4; j++) {
+                    x[j] *= exp2i(k);
+                    sum += x[j];
+                    const __half f = __float2half_rn(x[j] * ((j & 1) ? 0x1p-4f : 1.f));
+                    dst[j * 128] = __half_as_ushort(f);
+                }
+            }
+#pragma unroll
+            for (int i = 1; i < 16; i <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, i);
+            if (lane % 16 == 0 && lane < D / 4) sm_qs[lane / 16][col] = sum * 0x1p-24f;
+            if (lane == 0) sm_cf[col] = a.c * exp2i(24 - k);
+        }
+        __syncthreads();
+        const int first_ids = next.any ? fetch_ids(next, 0) : -1;
         uint32_t qf[NT][NG][4][2];
         float cf[NT][2], qs[NT][NG][2];
         int hi[NT][2], lo[NT][2];
         int min_hi = 0x7fffffff, max_lo = 0;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
-            const int n = n0 + 8 * nt + g;
-            float x[NG][16];
-            float amax = 0.f;
 #pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                uint4 w0 = make_uint4(0, 0, 0, 0), w1 = w0;
-                if (n < rows) {
-                    const int tok = n / a.group;
-                    const uint16_t* p = (const uint16_t*)a.q.data + (s.row0 + tok) * a.q.st +
-                                        (at.head * a.group + n - tok * a.group) * a.q.sh + gr * KV4_GROUP + 16 * c;
-                    w0 = ((const uint4*)p)[0];
-                    w1 = ((const uint4*)p)[1];
-                }
-                unpack_bf16x8(w0, x[gr]);
-                unpack_bf16x8(w1, x[gr] + 8);
-#pragma unroll
-                for (int i = 0; i < 16; i++) amax = fmaxf(amax, fabsf(x[gr][i]));
-            }
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-            amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-            // 2^k brings the row's largest magnitude to [2^13, 2^14)
-            const int e = (int)(__float_as_uint(amax) >> 23) - 127;
-            const int k = min(max(13 - e, -100), 100);
-            const float up = __uint_as_float((uint32_t)(k + 127) << 23);
-            float sum[NG];
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                sum[gr] = 0.f;
-#pragma unroll
-                for (int i = 0; i < 16; i++) {
-                    x[gr][i] *= up;
-                    sum[gr] += x[gr][i];
-                }
+            for (int gr = 0; gr < NG; gr++)
 #pragma unroll
                 for (int j = 0; j < 4; j++) {
-                    const float f = (j & 1) ? 0x1p-4f : 1.f;
-                    const __half2 h0 = __floats2half2_rn(x[gr][j] * f, x[gr][4 + j] * f);
-                    const __half2 h1 = __floats2half2_rn(x[gr][8 + j] * f, x[gr][12 + j] * f);
-                    qf[nt][gr][j][0] = *(const uint32_t*)&h0;
-                    qf[nt][gr][j][1] = *(const uint32_t*)&h1;
+                    const uint2 w = ((const uint2*)sm_q)[((nt * NG + gr) * 4 + j) * 32 + lane];
+                    qf[nt][gr][j][0] = w.x;
+                    qf[nt][gr][j][1] = w.y;
                 }
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 1);
-                sum[gr] += __shfl_xor_sync(0xffffffffu, sum[gr], 2);
-            }
-            const float down = a.c * __uint_as_float((uint32_t)(24 - k + 127) << 23);
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                cf[nt][j] = __shfl_sync(0xffffffffu, down, 4 * (2 * c + j));
+                const int col = 8 * nt + 2 * c + j, tok = by_group(a, min(n0 + col, rows - 1));
+                cf[nt][j] = sm_cf[col];
 #pragma unroll
-                for (int gr = 0; gr < NG; gr++)
-                    qs[nt][gr][j] = __shfl_sync(0xffffffffu, sum[gr], 4 * (2 * c + j)) * 0x1p-24f;
-                const int m = n0 + 8 * nt + 2 * c + j, tok = min(m, rows - 1) / a.group;
+                for (int gr = 0; gr < NG; gr++) qs[nt][gr][j] = sm_qs[gr][col];
                 hi[nt][j] = key_hi(a, s, tok);
                 lo[nt][j] = key_lo(a, s, tok);
                 min_hi = min(min_hi, hi[nt][j]);
@@ -278,8 +434,15 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
         }
         min_hi = __reduce_min_sync(0xffffffffu, min_hi);
         max_lo = __reduce_max_sync(0xffffffffu, max_lo);
+        const int all_hi = min(min_hi, k1);
 
-        float m[NT][2], l[NT][2], zs[NT][NG][2], o[NT][NG][MT][4], ones[NT][NG][4];
+        float m[NT][2], l[NT][2], zs[NT][NG][2], o[NT][NG][MT][4];
+        float v_up[NG], v_lim[NG];  // 2^(14 - R), 2^(R + 1)
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) {
+            v_up[gr] = 1.f;
+            v_lim[gr] = -1.f;
+        }
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -292,21 +455,26 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
             for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    ones[nt][gr][i] = 0.f;
+                for (int i = 0; i < 4; i++)
 #pragma unroll
                     for (int t = 0; t < MT; t++) o[nt][gr][t][i] = 0.f;
-                }
         }
 
         // ---- the warp's steps
         for (int i = 0; i < steps; i++) {
             cp_wait<C::STAGES - 2>();
             __syncwarp();
-            issue(i + C::STAGES - 1);
-            const uint32_t st = ring + (i % C::STAGES) * C::STAGE;
+            issue(p, i + C::STAGES - 1, steps);
+            const uint32_t st = ring + stage * C::STAGE;
+            uint32_t k_at[NG], v_at[2];
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) k_at[gr] = st + k_off[gr];
+            v_at[0] = st + v_off[0];
+            v_at[1] = st + v_off[1];
+            const uint32_t p_at = st + p_off;
+            stage = stage + 1 == C::STAGES ? 0 : stage + 1;
             const int key0 = k0 + (i * AT_WARPS + warp) * AT_STEP;
-            const bool edge = key0 + AT_STEP > min(min_hi, k1) || key0 < max_lo;
+            const bool edge = key0 + AT_STEP > all_hi || key0 < max_lo;
             float x[2][NT][4];  // [16 keys][columns][C fragment]: S, then P
             float vs[2][2][NG], vz[2][2][NG];
 #pragma unroll
@@ -316,12 +484,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
                 float acc[NG][NT][4];
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
-                    const uint2 wl = lds64(st + stage_at<D>(kl, gr * 32 + c * 8));
-                    const uint2 wh = lds64(st + stage_at<D>(kl + 8, gr * 32 + c * 8));
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                        for (int q = 0; q < 4; q++) acc[gr][nt][q] = 0.f;
+                    const uint2 wl = lds64(k_at[gr] + h * (C::VAL / 2));
+                    const uint2 wh = lds64(k_at[gr] + h * (C::VAL / 2) + C::VAL / 4);
 #pragma unroll
                     for (int j = 0; j < 4; j++) {
                         const int sh = j >= 2 ? 8 : 0;
@@ -329,12 +493,16 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
                         const uint32_t f[4] = {(wl.x >> sh) & mask, (wh.x >> sh) & mask, (wl.y >> sh) & mask,
                                                (wh.y >> sh) & mask};
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_f16(acc[gr][nt], f, qf[nt][gr][j][0], qf[nt][gr][j][1]);
+                        for (int nt = 0; nt < NT; nt++)
+                            if (j == 0)
+                                mma_f16_0(acc[gr][nt], f, qf[nt][gr][j][0], qf[nt][gr][j][1]);
+                            else
+                                mma_f16(acc[gr][nt], f, qf[nt][gr][j][0], qf[nt][gr][j][1]);
                     }
                 }
 #pragma unroll
                 for (int r = 0; r < 2; r++) {
-                    const uint32_t par = st + 2 * C::VAL + (kl + 8 * r) * (NG * 4);
+                    const uint32_t par = p_at + (16 * h + 8 * r) * (NG * 4);
                     uint32_t kp[NG], vp[NG];
                     if constexpr (NG == 2) {
                         const uint2 t = lds64(par), w = lds64(par + C::PAR);
@@ -346,7 +514,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++) {
                         vs[h][r][gr] = bf_lo(vp[gr]);
-                        vz[h][r][gr] = fmaf(8.f, vs[h][r][gr], bf_hi(vp[gr]));
+                        vz[h][r][gr] = bf_hi(vp[gr]);
                     }
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
@@ -371,7 +539,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                         for (int gr = 0; gr < NG; gr++) {
                             bad[gr] = !(fabsf(vs[h][r][gr]) + fabsf(vz[h][r][gr]) < INFINITY);
-                            if (bad[gr]) vs[h][r][gr] = vz[h][r][gr] = 0.f;
+                            if (bad[gr] || key >= k1 || key < p.kr.first) vs[h][r][gr] = vz[h][r][gr] = 0.f;
                         }
 #pragma unroll
                         for (int nt = 0; nt < NT; nt++)
@@ -413,7 +581,6 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                         for (int gr = 0; gr < NG; gr++) {
                             zs[nt][gr][j] *= f;
-                            ones[nt][gr][j] *= f;
 #pragma unroll
                             for (int t = 0; t < MT; t++) {
                                 o[nt][gr][t][j] *= f;
@@ -427,6 +594,32 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
             for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) mc[nt][j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j] * cf[nt][j];
+
+            // ---- V's scales within f16's reach
+            float top[NG];
+            bool over = false;
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                top[gr] = fmaxf(fmaxf(vs[0][0][gr], vs[0][1][gr]), fmaxf(vs[1][0][gr], vs[1][1][gr]));
+                over = over || top[gr] > v_lim[gr];
+            }
+            if (__any_sync(0xffffffffu, over)) {
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top[gr])));
+                    if (!(most > v_lim[gr])) continue;
+                    const int R = max((int)(__float_as_uint(most) >> 23) - 126, -100);  // most < 2^R
+                    const float up = exp2i(14 - R), f = up / v_up[gr];
+                    v_lim[gr] = exp2i(min(R + 1, 127));
+                    v_up[gr] = up;
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int t = 0; t < MT; t++)
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; i4++) o[nt][gr][t][i4] *= f;
+                }
+            }
 
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -447,72 +640,75 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++)
 #pragma unroll
-                        for (int r = 0; r < 2; r++)
-                            pf[nt][gr][r] = transpose8(pack_bf16x2(x[h][nt][2 * r] * vs[h][r][gr],
-                                                                   x[h][nt][2 * r + 1] * vs[h][r][gr]));
+                        for (int r = 0; r < 2; r++) {
+                            const float sc = vs[h][r][gr] * v_up[gr];
+                            pf[nt][gr][r] = transpose8(pack_f16x2(x[h][nt][2 * r] * sc, x[h][nt][2 * r + 1] * sc));
+                        }
                 }
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
                     uint32_t w[4];  // 8 channels of keys c, c + 4, c + 8, c + 12
 #pragma unroll
                     for (int i4 = 0; i4 < 4; i4++)
-                        w[i4] = lds32(st + C::VAL + stage_at<D>(16 * h + c + 4 * i4, gr * 32 + g * 4));
-                    uint32_t up[4], dn[4];
+                        w[i4] = lds32(v_at[D == 128 ? (gr + i4) & 1 : i4 & 1] + h * (C::VAL / 2) + 4 * i4 * C::ROW);
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; i4++) {
-                        up[i4] = w[i4] << 3;
-                        dn[i4] = w[i4] >> 1;
-                    }
-#pragma unroll
-                    for (int t = 0; t < MT; t++) {  // channels 8g + 2t (row g) and 8g + 2t + 1 (row g + 8)
+                    for (int t = 0; t < MT; t++) {  // channels 8g + 2t (row g, 2^-24) and 8g + 2t + 1 (row g + 8, 2^-20)
                         const uint32_t sel = t | (t << 4) | ((4 + t) << 8) | ((4 + t) << 12);
-                        const uint32_t f[4] = {(__byte_perm(up[0], up[1], sel) & 0x00780078u) | 0x41804180u,
-                                               (__byte_perm(dn[0], dn[1], sel) & 0x00780078u) | 0x41804180u,
-                                               (__byte_perm(up[2], up[3], sel) & 0x00780078u) | 0x41804180u,
-                                               (__byte_perm(dn[2], dn[3], sel) & 0x00780078u) | 0x41804180u};
+                        const uint32_t y0 = __byte_perm(w[0], w[1], sel), y1 = __byte_perm(w[2], w[3], sel);
+                        const uint32_t f[4] = {y0 & 0x000f000fu, y0 & 0x00f000f0u, y1 & 0x000f000fu, y1 & 0x00f000f0u};
 #pragma unroll
-                        for (int nt = 0; nt < NT; nt++) mma_bf16(o[nt][gr][t], f, pf[nt][gr][0], pf[nt][gr][1]);
+                        for (int nt = 0; nt < NT; nt++) mma_f16(o[nt][gr][t], f, pf[nt][gr][0], pf[nt][gr][1]);
                     }
-                    const uint32_t one[4] = {0x3f803f80u, 0x3f803f80u, 0x3f803f80u, 0x3f803f80u};
-#pragma unroll
-                    for (int nt = 0; nt < NT; nt++) mma_bf16(ones[nt][gr], one, pf[nt][gr][0], pf[nt][gr][1]);
                 }
             }
         }
         cp_wait<0>();
         __syncwarp();
+        if (next.any) {
+            cur_ids = first_ids;
+            begin(next);
+        }
 
-        // ---- the warps' outputs meet: own = acc - 24 sum(p s) + sum(p (z + 8 s))
+        // ---- the warps' outputs meet: acc * 2^24 / 2^(14 - R) + sum(p z),
+        // stored [group][channel within 8][g][column], without bank conflicts
 #pragma unroll
-        for (int nt = 0; nt < NT; nt++)
+        for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+            for (int gr = 0; gr < NG; gr++) {
+                float z[2];
+                const float back = 1.f / v_up[gr];  // 2^(R - 14)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    z[j] = zs[nt][gr][j];
+#pragma unroll
+                    for (int i = 4; i < 32; i <<= 1) z[j] += __shfl_xor_sync(0xffffffffu, z[j], i);
+                }
+#pragma unroll
+                for (int t = 0; t < MT; t++)
+#pragma unroll
+                    for (int r = 0; r < 2; r++)
+                        *(float2*)(sm_o + ((nt * NG + gr) * 64 + (2 * t + r) * 8 + g) * 8 + 2 * c) =
+                            make_float2(fmaf(o[nt][gr][t][2 * r] * (r ? 0x1p20f : 0x1p24f), back, z[0]),
+                                        fmaf(o[nt][gr][t][2 * r + 1] * (r ? 0x1p20f : 0x1p24f), back, z[1]));
+            }
 #pragma unroll
             for (int j = 0; j < 2; j++) {
-                const int col = 8 * nt + 2 * c + j;
-                float z[NG], ls = l[nt][j];
+                float ls = l[nt][j];
 #pragma unroll
                 for (int i = 4; i < 32; i <<= 1) ls += __shfl_xor_sync(0xffffffffu, ls, i);
-#pragma unroll
-                for (int gr = 0; gr < NG; gr++) {
-                    z[gr] = zs[nt][gr][j];
-#pragma unroll
-                    for (int i = 4; i < 32; i <<= 1) z[gr] += __shfl_xor_sync(0xffffffffu, z[gr], i);
-                    z[gr] -= 24.f * ones[nt][gr][j];
-#pragma unroll
-                    for (int t = 0; t < MT; t++) {
-                        float2 v = make_float2(o[nt][gr][t][j] + z[gr], o[nt][gr][t][2 + j] + z[gr]);
-                        *(float2*)(sm_o + col * D + gr * KV4_GROUP + 8 * g + 2 * t) = v;
-                    }
-                }
                 if (g == 0) {
-                    sm_m[warp][col] = m[nt][j] == -INFINITY ? -INFINITY : m[nt][j] * cf[nt][j];
-                    sm_l[warp][col] = ls;
+                    sm_m[warp][8 * nt + 2 * c + j] = m[nt][j] == -INFINITY ? -INFINITY : m[nt][j] * cf[nt][j];
+                    sm_l[warp][8 * nt + 2 * c + j] = ls;
                 }
             }
+        }
         __syncthreads();
-        const bool whole = u == at.start && piece_end == tile_end;
-        const int slot = 2 * (int)blockIdx.x + (at.start < u_begin ? 0 : 1);
+        const bool whole = p.unit0 == 0 && p.unit1 == p.kr.units;
+        const int slot = 2 * (int)blockIdx.x + (p.unit0 ? 0 : 1);
         for (int i = threadIdx.x; i < COLS * D / 4; i += blockDim.x) {
-            const int col = i / (D / 4), d4 = i % (D / 4) * 4, n = n0 + col;
+            // column, g, half of the 8 channels, group, nt
+            const int half = i >> 6 & 1, part = i >> 7, col = 8 * (part / NG) + (i & 7), n = n0 + col;
+            const int d4 = part % NG * KV4_GROUP + 8 * (i >> 3 & 7) + 4 * half;
             if (n >= rows) continue;
             float mm = -INFINITY;
 #pragma unroll
@@ -523,107 +719,61 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
             for (int w = 0; w < AT_WARPS; w++) {
                 const float f = ex2(sm_m[w][col] - ref);
-                const float4 y = *(const float4*)((const float*)(smem + w * C::WARP) + col * D + d4);
+                const float* y = (const float*)(smem + w * C::WARP + C::OUT) + part * 512 + half * 256 + (i & 63);
                 sum = fmaf(f, sm_l[w][col], sum);
-                v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
-                v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+                v.x = fmaf(f, y[0], v.x); v.y = fmaf(f, y[64], v.y);
+                v.z = fmaf(f, y[128], v.z); v.w = fmaf(f, y[192], v.w);
             }
             if (whole) {
-                put_row<D>(a, s, at.head, n, d4, v, ref, sum);
+                put_row<D>(a, s, p.at.head, n, d4, v, ref, sum);
             } else {
                 *(float4*)(a.part_o + ((long long)slot * COLS + col) * D + d4) = v;
                 if (d4 == 0) a.part_ml[slot * COLS + col] = make_float2(mm, sum);
             }
         }
         __syncthreads();
-
-        // ---- the next tile
-        u = piece_end;
-        if (u < u_end) {
-            at.start = tile_end;
-            if (++at.tile >= s.tiles) {
-                at.tile = 0;
-                if (++at.head >= a.pool.kv_heads) {
-                    at.head = 0;
-                    do at.b++;
-                    while (at.b < a.batch && seq_at<COLS>(a, at.b).tiles == 0);
-                }
+        if (!whole) {
+            // ---- a piece of a split tile: the last to finish joins them
+            const int c0 = p.unit0 ? sh.holder(p.at.start) : blockIdx.x;
+            const int c1 = p.unit1 < p.kr.units ? sh.holder(p.at.start + p.kr.units - 1) : blockIdx.x;
+            if (threadIdx.x == 0) {
+                // (releases the whole CTA's writes, which the barrier ordered before; acquires the others')
+                uint32_t n;
+                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(a.done + c0) : "memory");
+                sm_last = n == (uint32_t)(c1 - c0);
+                if (sm_last) a.done[c0] = 0;
             }
+            __syncthreads();
+            if (sm_last)
+                join_tile<D, COLS, C::WARP>(a, s, p.at.head, n0, min(COLS, rows - n0), c0, c1, smem + C::OUT, sm_join);
         }
+        if (!next.any) return;
     }
 }
 
-// Joins the pieces of split tiles: block (c, column) joins that column of the
-// tile that begins in CTA c and ends in a later one.  A thread holds 4
-// channels of every (128 / (D/4))-th piece.
-template <int D, int COLS, int UNIT>
-__global__ void __launch_bounds__(128) sp_kv4_join(const __grid_constant__ Kv4Attend a) {
-    constexpr int LANES = D / 4, SLICES = 128 / LANES;
-    __shared__ float4 sm_v[SLICES][LANES];
-    __shared__ float2 sm_ml[SLICES];
-    const int col = blockIdx.y, lane = threadIdx.x % LANES, slice = threadIdx.x / LANES;
-    long long total, none;
-    count_units<COLS, UNIT>(a, 0, total, none);
-    total *= a.pool.kv_heads;
-    const int G = shares(total, gridDim.x);
-    if ((int)blockIdx.x >= G) return;
-    const long long u0 = first_unit(blockIdx.x, total, G), u1 = first_unit(blockIdx.x + 1, total, G);
-    const Place at = find_unit<COLS, UNIT>(a, u1 - 1);
-    const Seq s = seq_at<COLS>(a, at.b);
-    const long long end = at.start + keys_of<COLS, UNIT>(a, s, at.tile).units;
-    const int n = at.tile * COLS + col;
-    if (at.start < u0 || end <= u1 || n >= s.qn * a.group) return;
-    const int c0 = blockIdx.x, c1 = cta_of(end - 1, total, G);
-    griddep_wait();
-    float m = -INFINITY, sum = 0.f;
-    float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int c = c0 + slice; c <= c1; c += SLICES) m = fmaxf(m, a.part_ml[(2 * c + (c == c0)) * COLS + col].x);
-    const float own_ref = m == -INFINITY ? 0.f : m;
-#pragma unroll 4
-    for (int c = c0 + slice; c <= c1; c += SLICES) {
-        const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
-        const float2 ml = a.part_ml[slot];
-        const float4 y = *(const float4*)(a.part_o + slot * D + 4 * lane);
-        const float f = ex2(ml.x - own_ref);
-        sum = fmaf(f, ml.y, sum);
-        v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
-        v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
-    }
-    sm_v[slice][lane] = v;
-    if (lane == 0) sm_ml[slice] = make_float2(m, sum);
-    __syncthreads();
-    if (slice) return;
-    float mm = -INFINITY;
-#pragma unroll
-    for (int i = 0; i < SLICES; i++) mm = fmaxf(mm, sm_ml[i].x);
-    const float ref = mm == -INFINITY ? 0.f : mm;
-    sum = 0.f;
-    v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int i = 0; i < SLICES; i++) {
-        const float f = ex2(sm_ml[i].x - ref);
-        const float4 y = sm_v[i][lane];
-        sum = fmaf(f, sm_ml[i].y, sum);
-        v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
-        v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
-    }
-    put_row<D>(a, s, at.head, n, 4 * lane, v, ref, sum);
+size_t kv4_scratch_bytes(int d, int sms) {
+    return KV4_COUNTS + (size_t)2 * sms * 16 * (d + 2) * sizeof(float);
 }
-
-size_t kv4_scratch_bytes(int d, int sms) { return (size_t)2 * 2 * sms * 16 * (d + 2) * sizeof(float); }
 
 template <int D, int NT>
 static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
     using C = AttnCfg<D, NT>;
     constexpr int COLS = C::COLS;
     const int G = (NT == 1 ? 2 : 1) * sms;
-    a.part_ml = (float2*)a.scratch;
+    if (G * sizeof(uint32_t) > KV4_COUNTS) return cudaErrorInvalidConfiguration;
+    a.done = (uint32_t*)a.scratch;
+    a.part_ml = (float2*)((uint8_t*)a.scratch + KV4_COUNTS);
     a.part_o = (float*)(a.part_ml + (size_t)2 * G * COLS);
-    cudaError_t e = cudaFuncSetAttribute(sp_kv4_attend<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+    static std::atomic<uint64_t> ready{0};  // devices whose limit of shared memory is raised, one bit each
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
-    sp_kv4_attend<D, NT><<<G, AT_WARPS * 32, C::SMEM, st>>>(a);
-    if ((e = cudaGetLastError()) != cudaSuccess) return e;
-    return launch_after_previous(sp_kv4_join<D, COLS, AT_UNIT>, dim3(G, COLS), dim3(128), 0, st, a);
+    if (!(ready.load() >> (dev & 63) & 1)) {
+        e = cudaFuncSetAttribute(sp_kv4_attend<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        if (e != cudaSuccess) return e;
+        ready.fetch_or(1ull << (dev & 63));
+    }
+    return launch_after_previous(sp_kv4_attend<D, NT>, dim3(G), dim3(AT_WARPS * 32), C::SMEM, st, a);
 }
 
 cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t st) {

@@ -16,6 +16,7 @@
 // serves them all; the minimum and maximum of a group come from shuffles
 // among the D/16 lanes of a row.
 #include "rotary.cuh"
+#include "sage_kernels.h"
 
 namespace sp {
 
@@ -85,6 +86,8 @@ __global__ void __launch_bounds__(256) sp_kv4_append(const Kv4Pool pool, const R
                                                      int tokens, int q_heads, int row_blocks,
                                                      uint32_t* __restrict__ err) {
     constexpr int UNITS = D / 16, HL = 32 / UNITS, NG = D / KV4_GROUP;
+    griddep_wait();
+    griddep_launch_dependents();
     const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int t = (int)(w / row_blocks), rb = (int)(w % row_blocks);
     if (t >= tokens) return;
@@ -180,11 +183,8 @@ static cudaError_t append(const Kv4Pool& pool, const Rows& q, const Rows& q_out,
     const bool many = (long long)tokens * ((rows + 4 * HL - 1) / (4 * HL)) >= 148 * 16;
     const int per = many ? 4 : 1, rb = (rows + per * HL - 1) / (per * HL);
     const unsigned grid = (unsigned)(((long long)tokens * rb + 7) / 8);
-    if (many)
-        sp_kv4_append<D, 4><<<grid, 256, 0, st>>>(pool, q, q_out, k, v, r, slots, tokens, q_heads, rb, err);
-    else
-        sp_kv4_append<D, 1><<<grid, 256, 0, st>>>(pool, q, q_out, k, v, r, slots, tokens, q_heads, rb, err);
-    return cudaGetLastError();
+    return launch_after_previous(many ? sp_kv4_append<D, 4> : sp_kv4_append<D, 1>, dim3(grid), dim3(256), 0, st, pool, q,
+                                 q_out, k, v, r, slots, tokens, q_heads, rb, err);
 }
 
 cudaError_t launch_kv4_append(int d, const Kv4Pool& pool, const Rows& q, const Rows& q_out, const Rows& k,
@@ -201,6 +201,8 @@ template <int D>
 __global__ void __launch_bounds__(256) sp_kv4_read(const Kv4Pool pool, const int* __restrict__ slots, const Rows k,
                                                    const Rows v, int tokens, uint32_t* __restrict__ err) {
     constexpr int CH = D / 8, NG = D / KV4_GROUP;
+    griddep_wait();
+    griddep_launch_dependents();
     const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
     const int c = (int)(i % CH);
     const long long rowi = i / CH;
@@ -237,11 +239,8 @@ cudaError_t launch_kv4_read(int d, const Kv4Pool& pool, const int* slots, const 
                             uint32_t* err, cudaStream_t st) {
     const long long n = (long long)tokens * 2 * pool.kv_heads * (d / 8);
     const unsigned grid = (unsigned)((n + 255) / 256);
-    if (d == 64)
-        sp_kv4_read<64><<<grid, 256, 0, st>>>(pool, slots, k, v, tokens, err);
-    else
-        sp_kv4_read<128><<<grid, 256, 0, st>>>(pool, slots, k, v, tokens, err);
-    return cudaGetLastError();
+    return launch_after_previous(d == 64 ? sp_kv4_read<64> : sp_kv4_read<128>, dim3(grid), dim3(256), 0, st, pool, slots,
+                                 k, v, tokens, err);
 }
 
 }  // namespace sp

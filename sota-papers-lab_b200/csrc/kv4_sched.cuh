@@ -4,13 +4,14 @@
 // n = token * group + query head of the group, counted within the sequence's
 // queries.  A tile reads one range of keys, cut into units of UNIT keys.  All
 // units of the call, in the order sequence, KV head, tile, unit, are divided
-// evenly among the CTAs: CTA i takes units [i U / G, (i + 1) U / G).  So a
-// batch of any lengths is balanced, one long sequence is split over the whole
-// GPU, and the division follows from the lengths alone (the result does not
-// depend on which CTA runs first).  A tile that one CTA holds whole is written
-// out by it; the pieces of a split one go to the CTA's two scratch slots
-// (slot 1: the tile begins in the CTA, slot 0: it began before) and are joined
-// by a second kernel.
+// evenly among the CTAs, each taking a run of them.  So a batch of any lengths
+// is balanced, one long sequence is split over the whole GPU, and the division
+// follows from the lengths alone.  A tile that one CTA holds whole is written
+// out by it; the pieces of a split one go to scratch, in one of their CTA's two
+// slots (1: the tile begins in the CTA, 0: it began before), and the CTA that
+// finishes last joins them, in their order (so the result does not depend on
+// which CTA that is).  Its count of finished pieces, under the tile's first
+// CTA's number, is zero again when it leaves.
 //
 // Lengths are read from device memory, so every index is checked here: what
 // is out of range is clamped and flagged in the error word.
@@ -33,6 +34,11 @@ struct KeyRange {
     int lo, hi;  // the keys read: [lo, hi), lo = first rounded down to a multiple of 32
     int units;
 };
+
+// n / group, without a division.
+__device__ __forceinline__ int by_group(const Kv4Attend& a, int n) {
+    return a.group_mul ? (int)(__umulhi((uint32_t)n, a.group_mul) >> a.group_shift) : n;
+}
 
 // `flag`: report what is out of range (one caller does, not all).
 template <int COLS>
@@ -70,7 +76,7 @@ __device__ __forceinline__ int key_lo(const Kv4Attend& a, const Seq& s, int i) {
 template <int COLS, int UNIT>
 __device__ __forceinline__ KeyRange keys_of(const Kv4Attend& a, const Seq& s, int tile) {
     KeyRange r;
-    const int first = tile * COLS / a.group, last = min(s.qn - 1, (tile * COLS + COLS - 1) / a.group);
+    const int first = by_group(a, tile * COLS), last = min(s.qn - 1, by_group(a, tile * COLS + COLS - 1));
     r.hi = key_hi(a, s, last);
     r.first = min(key_lo(a, s, first), r.hi);
     r.lo = r.first & ~31;
@@ -86,72 +92,91 @@ __device__ __forceinline__ long long seq_units(const Kv4Attend& a, const Seq& s)
     return n;
 }
 
-// The CTAs that get work: with fewer units than CTAs one unit each.
-__device__ __forceinline__ int shares(long long U, int ctas) { return (int)min(U, (long long)ctas); }
-// CTA c of G <= U begins at unit c U / G; the CTA that holds unit u.
-__device__ __forceinline__ long long first_unit(long long c, long long U, int G) { return c * U / G; }
-__device__ __forceinline__ int cta_of(long long u, long long U, int G) { return (int)(((u + 1) * G - 1) / U); }
-
-// One warp's walk over the sequences: the units of all sequences (one KV
-// head), and of those before sequence `upto`.
-template <int COLS, int UNIT>
-__device__ __forceinline__ void count_units(const Kv4Attend& a, int upto, long long& total, long long& before) {
-    const int lane = threadIdx.x & 31;
-    long long n = 0, m = 0;
-    for (int b = lane; b < a.batch; b += 32) {
-        const long long x = seq_units<COLS, UNIT>(a, seq_at<COLS>(a, b));
-        n += x;
-        if (b < upto) m += x;
+// U units over `ctas` CTAs: the first U mod G of the G = min(U, ctas) that get
+// work have one unit more than the others.
+struct Shares {
+    long long U, q, r;  // q = U / G, r = U mod G
+    int G;
+    Shares() = default;
+    __device__ __forceinline__ Shares(long long units, int ctas) {
+        U = units;
+        G = (int)min(U, (long long)ctas);
+        if (U < 1ll << 32) {  // a short division
+            q = G ? (uint32_t)U / (uint32_t)G : 0;
+        } else {
+            q = U / G;
+        }
+        r = U - q * G;
     }
-#pragma unroll
-    for (int i = 16; i; i >>= 1) {
-        n += __shfl_xor_sync(0xffffffffu, n, i);
-        m += __shfl_xor_sync(0xffffffffu, m, i);
+    __device__ __forceinline__ long long first(int c) const { return c * q + min((long long)c, r); }
+    __device__ __forceinline__ int holder(long long u) const {  // the CTA of unit u
+        const long long wide = r * (q + 1);
+        const long long x = u < wide ? u : u - wide, per = u < wide ? q + 1 : q;
+        const int base = u < wide ? 0 : (int)r;
+        return base + (x < 1ll << 32 ? (int)((uint32_t)x / (uint32_t)per) : (int)(x / per));
     }
-    total = n;
-    before = m;
-}
+};
 
-// Where unit u lies.
+// Where a unit lies.
 struct Place {
     int b, head, tile;
     long long start;  // the tile's first unit
+    Seq s;
 };
 
-// All lanes of a warp call it with the same u < all units.
+// A warp finds CTA `cta`'s share and the tile it begins in (all lanes get it).
+// Lane i holds the lengths of sequence 32 k + i, so up to 32 sequences take one
+// round of loads.  Returns false where the CTA has no work.
 template <int COLS, int UNIT>
-__device__ __forceinline__ Place find_unit(const Kv4Attend& a, long long u) {
+__device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas, Shares& sh, Place& p) {
     const int lane = threadIdx.x & 31, hkv = a.pool.kv_heads;
-    Place p = {0, 0, 0, 0};
-    long long base = 0;
-    for (int b0 = 0; b0 < a.batch; b0 += 32) {
+    // sequences b0 + lane, their units, and the units up to and with them (one KV head)
+    Seq s;
+    long long x, incl;
+    auto scan = [&](int b0) {
         const int b = b0 + lane;
-        const long long x = b < a.batch ? hkv * seq_units<COLS, UNIT>(a, seq_at<COLS>(a, b)) : 0;
-        long long incl = x;
+        s = b < a.batch ? seq_at<COLS>(a, b) : Seq{0, 0, 0, 0};
+        x = incl = seq_units<COLS, UNIT>(a, s);
 #pragma unroll
         for (int i = 1; i < 32; i <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, incl, i);
             if (lane >= i) incl += y;
         }
-        const unsigned over = __ballot_sync(0xffffffffu, base + incl > u);
-        if (over) {
-            const int w = __ffs(over) - 1;
+    };
+    long long total = 0;
+    for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {  // the first 32 last: they stay
+        scan(b0);
+        total += __shfl_sync(0xffffffffu, incl, 31);
+    }
+    sh = Shares(total * hkv, ctas);
+    if (cta >= sh.G) return false;
+    const long long u = sh.first(cta);
+    long long base = 0;
+    for (int b0 = 0;; b0 += 32) {
+        if (b0) scan(b0);
+        const unsigned over = __ballot_sync(0xffffffffu, base + incl * hkv > u);
+        if (over || b0 + 32 >= a.batch) {
+            const int w = over ? __ffs(over) - 1 : 0;  // (u < U: there is one)
             p.b = b0 + w;
-            const long long per = __shfl_sync(0xffffffffu, x, w) / hkv;
-            p.start = base + __shfl_sync(0xffffffffu, incl - x, w);
-            p.head = (int)((u - p.start) / per);
+            const long long per = __shfl_sync(0xffffffffu, x, w);
+            p.start = base + __shfl_sync(0xffffffffu, incl - x, w) * hkv;
+            p.s.row0 = __shfl_sync(0xffffffffu, s.row0, w);
+            p.s.qn = __shfl_sync(0xffffffffu, s.qn, w);
+            p.s.kv = __shfl_sync(0xffffffffu, s.kv, w);
+            p.s.tiles = __shfl_sync(0xffffffffu, s.tiles, w);
+            const long long off = u - p.start;
+            p.head = off < per ? 0 : off < 1ll << 32 ? (int)((uint32_t)off / (uint32_t)per) : (int)(off / per);
             p.start += p.head * per;
             break;
         }
-        base += __shfl_sync(0xffffffffu, incl, 31);
+        base += __shfl_sync(0xffffffffu, incl, 31) * hkv;
     }
-    const Seq s = seq_at<COLS>(a, p.b);
-    for (;; p.tile++) {
-        const int n = keys_of<COLS, UNIT>(a, s, p.tile).units;
-        if (u < p.start + n || p.tile + 1 >= s.tiles) break;
+    for (p.tile = 0; p.tile + 1 < p.s.tiles; p.tile++) {
+        const int n = keys_of<COLS, UNIT>(a, p.s, p.tile).units;
+        if (u < p.start + n) break;
         p.start += n;
     }
-    return p;
+    return true;
 }
 
 }  // namespace sp

@@ -8,6 +8,7 @@
 // with one head a thread the table (64 bytes for 32 bytes of bf16 channels)
 // would pass the L1 twice as often as the data.
 #include "rotary.cuh"
+#include "sage_kernels.h"
 
 namespace sp {
 
@@ -18,6 +19,8 @@ template <int D, int DT, int HPT>
 __global__ void __launch_bounds__(256) sp_rope(const Rows x, const Rows out, const RotaryArgs r, int tokens, int heads,
                                                int head_blocks, int backward, uint32_t* __restrict__ err) {
     constexpr int UNITS = D / 16, HL = 32 / UNITS;
+    griddep_wait();
+    griddep_launch_dependents();
     const long long w = (long long)blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32;
     const int t = (int)(w / head_blocks), hb = (int)(w % head_blocks);
     if (t >= tokens) return;
@@ -68,11 +71,8 @@ static cudaError_t rope(const Rows& x, const Rows& out, const RotaryArgs& r, int
     const int per = many ? 4 : 1, hb = (heads + per * HL - 1) / (per * HL);
     const long long warps = (long long)tokens * hb;
     const unsigned grid = (unsigned)((warps + 7) / 8);
-    if (many)
-        sp_rope<D, DT, 4><<<grid, 256, 0, st>>>(x, out, r, tokens, heads, hb, backward, err);
-    else
-        sp_rope<D, DT, 1><<<grid, 256, 0, st>>>(x, out, r, tokens, heads, hb, backward, err);
-    return cudaGetLastError();
+    return launch_after_previous(many ? sp_rope<D, DT, 4> : sp_rope<D, DT, 1>, dim3(grid), dim3(256), 0, st, x, out, r,
+                                 tokens, heads, hb, backward, err);
 }
 
 cudaError_t launch_rope(int d, int dtype, const Rows& x, const Rows& out, const RotaryArgs& r, int tokens, int heads,
