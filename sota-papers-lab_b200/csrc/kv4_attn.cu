@@ -30,6 +30,7 @@
 // shared memory (cp.async, 16 bytes, no barrier but the warp's own) with its
 // own running maximum and sums; the warps meet once per tile.  Row maxima are
 // looked at by vote and only recomputed when one grows.
+#include <algorithm>
 #include <atomic>
 
 #include "kv4_sched.cuh"
@@ -38,6 +39,9 @@
 namespace sp {
 
 constexpr int AT_WARPS = 8, AT_STEP = 32, AT_UNIT = 128;
+// Units a CTA takes at least: all 8 warps get a step (200 cached tokens: 7.0 us
+// instead of 8.6 with 1, 9.8 with 4; 1000: 10.0, 9.2, 11.8).
+constexpr int AT_LEAST = 2;
 
 template <int D, int NT>
 struct AttnCfg {
@@ -145,123 +149,6 @@ __device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, co
     }
 }
 
-// The part of a tile that a CTA works on: its units unit0 .. unit1 - 1.
-struct Piece {
-    Place at;
-    KeyRange kr;
-    int unit0, unit1;
-    bool any;  // there is such a piece
-};
-
-template <int COLS>
-__device__ __forceinline__ void cut_piece(const Kv4Attend& a, const Shares& sh, long long from, Piece& p) {
-    p.kr = keys_of<COLS, AT_UNIT>(a, p.at.s, p.at.tile);
-    p.unit0 = (int)(from - p.at.start);
-    p.unit1 = (int)min((long long)p.kr.units, sh.first(blockIdx.x + 1) - p.at.start);
-}
-
-// The piece after p in the CTA's share.
-template <int COLS>
-__device__ __forceinline__ void next_piece(const Kv4Attend& a, const Shares& sh, const Piece& p, Piece& n) {
-    n.any = p.at.start + p.unit1 < sh.first(blockIdx.x + 1);
-    if (!n.any) return;
-    n.at = p.at;
-    n.at.start += p.kr.units;
-    if (++n.at.tile >= n.at.s.tiles) {
-        n.at.tile = 0;
-        if (++n.at.head >= a.pool.kv_heads) {
-            n.at.head = 0;
-            do n.at.s = seq_at<COLS>(a, ++n.at.b);  // (units are left: there is one)
-            while (n.at.s.tiles == 0);
-        }
-    }
-    cut_piece<COLS>(a, sh, n.at.start, n);
-}
-
-// Four channels of row n of the sequence, from sums relative to 2^ref.  A row
-// that saw no key (sum 0) is written as zeros, its lse as -infinity.
-template <int D>
-__device__ __forceinline__ void put_row(const Kv4Attend& a, const Seq& s, int kv_head, int n, int d, float4 v, float ref,
-                                        float sum) {
-    const int tok = by_group(a, n), head = kv_head * a.group + n - tok * a.group;
-    const float inv = 1.f / sum;
-    uint2 r = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
-    if (sum == 0.f) r = make_uint2(0u, 0u);
-    *(uint2*)((uint16_t*)a.out.data + (s.row0 + tok) * a.out.st + head * a.out.sh + d) = r;
-    if (a.lse && d == 0)
-        a.lse[(long long)(s.row0 + tok) * a.heads + head] = (ref + log2f(sum)) * 0.6931471805599453f;
-}
-
-// Joins the pieces that CTAs c0 .. c1 left of a tile's `cols` columns from row
-// n0 on.  D/4 threads hold a column's channels; where columns are few, the
-// pieces of one are shared out among several such teams, which meet in `sm`
-// (each warp's output area, WARP bytes apart) and `sm_ml`.
-template <int D, int COLS, int WARP>
-__device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int head, int n0, int cols, int c0, int c1,
-                                          uint8_t* sm, float2* sm_ml) {
-    constexpr int LANES = D / 4, TEAMS = AT_WARPS * 32 / LANES;
-    const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
-    int slices = 1;
-    while (2 * slices * cols <= TEAMS) slices *= 2;
-    const int per = TEAMS / slices, slice = team / per;  // columns at a time
-    auto sm_v = [&](int t) { return (float4*)(sm + t * LANES / 32 * WARP) + t * LANES % 32 + lane; };
-    for (int first = 0; first < cols; first += per) {
-        const int col = first + team % per;
-        float m = -INFINITY, sum = 0.f;
-        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-        // a few pieces at a time, all of their loads under way before the first is used
-        constexpr int AHEAD = 8;
-        for (int b = c0 + slice; b <= c1; b += slices * AHEAD) {
-            float2 ml[AHEAD];
-            float4 y[AHEAD];
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const int c = b + i * slices;
-                ml[i] = make_float2(-INFINITY, 0.f);
-                y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                if (c <= c1 && col < cols) {
-                    const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
-                    ml[i] = __ldcg(&a.part_ml[slot]);
-                    y[i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
-                }
-            }
-            const float old = m;
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) m = fmaxf(m, ml[i].x);
-            const float ref = m == -INFINITY ? 0.f : m, f0 = ex2(old - ref);
-            sum *= f0;
-            v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
-#pragma unroll
-            for (int i = 0; i < AHEAD; i++) {
-                const float f = ex2(ml[i].x - ref);
-                sum = fmaf(f, ml[i].y, sum);
-                v.x = fmaf(f, y[i].x, v.x); v.y = fmaf(f, y[i].y, v.y);
-                v.z = fmaf(f, y[i].z, v.z); v.w = fmaf(f, y[i].w, v.w);
-            }
-        }
-        *sm_v(team) = v;
-        if (lane == 0) sm_ml[team] = make_float2(m, sum);
-        __syncthreads();
-        if (slice == 0 && col < cols) {
-            float mm = -INFINITY;
-            for (int i = 0; i < slices; i++) mm = fmaxf(mm, sm_ml[team + i * per].x);
-            const float ref = mm == -INFINITY ? 0.f : mm;
-            sum = 0.f;
-            v = make_float4(0.f, 0.f, 0.f, 0.f);
-            for (int i = 0; i < slices; i++) {
-                const float2 ml = sm_ml[team + i * per];
-                const float4 y = *sm_v(team + i * per);
-                const float f = ex2(ml.x - ref);
-                sum = fmaf(f, ml.y, sum);
-                v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
-                v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
-            }
-            put_row<D>(a, s, head, n0 + col, 4 * lane, v, ref, sum);
-        }
-        __syncthreads();
-    }
-}
-
 template <int D, int NT>
 __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(const __grid_constant__ Kv4Attend a) {
     using C = AttnCfg<D, NT>;
@@ -297,8 +184,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
     if (warp == 0) {
         Shares share;
         Piece p;
-        p.any = find_share<COLS, AT_UNIT>(a, blockIdx.x, gridDim.x, share, p.at);
-        if (p.any) cut_piece<COLS>(a, share, share.first(blockIdx.x), p);
+        p.any = find_share<COLS, AT_UNIT, AT_LEAST>(a, blockIdx.x, gridDim.x, share, p.at);
+        if (p.any) cut_piece<COLS, AT_UNIT>(a, share, share.first(blockIdx.x), p);
         if (lane == 0) {
             sh = share;
             pieces[0] = p;
@@ -321,7 +208,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
         if (key < end_key(p) && key + 16 > p.kr.first) {
             id = a.pages[(long long)p.at.b * a.max_pages + (key >> a.pool.page_shift)];
             if (id < 0 || id >= a.pool.pages) {
-                atomicOr(a.err, ERR_INDEX);
+                atomicOr(a.err + ERR_INDEX_WORD, ERR_INDEX);
                 id = -1;
             }
         }
@@ -373,7 +260,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
         const Seq s = p.at.s;
         const int k0 = first_key(p), k1 = end_key(p), steps = steps_of(k0, k1);
         const int n0 = p.at.tile * COLS, rows = s.qn * a.group;
-        if (threadIdx.x == blockDim.x - 1) next_piece<COLS>(a, sh, p, next);
+        if (threadIdx.x == blockDim.x - 1) next_piece<COLS, AT_UNIT>(a, sh, p, next);
 
         // ---- the query rows as B fragments, column by column: channel 16c +
         // 4i + j of a group is half-word i of lane c's fragment j, the order
@@ -736,23 +623,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
             // ---- a piece of a split tile: the last to finish joins them
             const int c0 = p.unit0 ? sh.holder(p.at.start) : blockIdx.x;
             const int c1 = p.unit1 < p.kr.units ? sh.holder(p.at.start + p.kr.units - 1) : blockIdx.x;
-            if (threadIdx.x == 0) {
-                // (releases the whole CTA's writes, which the barrier ordered before; acquires the others')
-                uint32_t n;
-                asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(a.done + c0) : "memory");
-                sm_last = n == (uint32_t)(c1 - c0);
-                if (sm_last) a.done[c0] = 0;
-            }
+            if (threadIdx.x == 0) sm_last = last_piece(a, c0, c1);
             __syncthreads();
             if (sm_last)
-                join_tile<D, COLS, C::WARP>(a, s, p.at.head, n0, min(COLS, rows - n0), c0, c1, smem + C::OUT, sm_join);
+                join_tile<D, COLS, AT_WARPS * 32, C::WARP>(a, s, p.at.head, n0, min(COLS, rows - n0), c0, c1, smem + C::OUT, sm_join);
         }
         if (!next.any) return;
     }
 }
 
 size_t kv4_scratch_bytes(int d, int sms) {
-    return KV4_COUNTS + (size_t)2 * sms * 16 * (d + 2) * sizeof(float);
+    return std::max(KV4_COUNTS + (size_t)2 * sms * 16 * (d + 2) * sizeof(float), kv4_prompt_scratch_bytes(d, sms));
 }
 
 template <int D, int NT>
@@ -778,6 +659,12 @@ static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
 
 cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t st) {
     const int rows = a.max_q * a.group;
+    // Above 128 rows the tensor-core kernel with a tile of up to 256 rows, up
+    // to there this one's tiles of 16 (which read the cache again from the L2).
+    // 8 sequences, window 8192, 32 / 8 heads, D = 128, us here and there: 20
+    // rows 43 and 105, 64 rows 65 and 108, 128 rows 110 and 113, 256 rows 201
+    // and 131; one sequence of 2000 tokens, 128 rows: 19 and 54.
+    if (rows > 128) return launch_kv4_prompt(d, a, sms, st);
     if (d == 64) return rows <= 8 ? attend<64, 1>(a, sms, st) : attend<64, 2>(a, sms, st);
     return rows <= 8 ? attend<128, 1>(a, sms, st) : attend<128, 2>(a, sms, st);
 }

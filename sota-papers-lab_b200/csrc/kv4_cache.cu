@@ -106,7 +106,7 @@ __global__ void __launch_bounds__(256) sp_kv4_append(const Kv4Pool pool, const R
     const int slot = slots[t];
     const int page = slot >> pool.page_shift;
     if (!ok || page >= pool.pages) {  // the token is left out
-        if (lane == 0) atomicOr(err, ERR_INDEX);
+        if (lane == 0) atomicOr(err + ERR_INDEX_WORD, ERR_INDEX);
         return;
     }
     Chunk<0> lo[HPT], hi[HPT];
@@ -213,7 +213,7 @@ __global__ void __launch_bounds__(256) sp_kv4_read(const Kv4Pool pool, const int
     const int slot = slots[t];
     const int page = slot >> pool.page_shift;
     if (page >= pool.pages) {
-        if (c == 0 && row == 0) atomicOr(err, ERR_INDEX);
+        if (c == 0 && row == 0) atomicOr(err + ERR_INDEX_WORD, ERR_INDEX);
         return;
     }
     const bool is_v = row >= pool.kv_heads;

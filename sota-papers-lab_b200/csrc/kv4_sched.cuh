@@ -59,7 +59,7 @@ __device__ __forceinline__ Seq seq_at(const Kv4Attend& a, int b, bool flag = fal
     const long long most = (long long)a.max_pages << a.pool.page_shift;
     s.kv = (int)min((long long)max(n, 0), most);
     ok = ok && s.kv == n;
-    if (flag && !ok) atomicOr(a.err, ERR_INDEX);
+    if (flag && !ok) atomicOr(a.err + ERR_INDEX_WORD, ERR_INDEX);
     s.tiles = (s.qn * a.group + COLS - 1) / COLS;
     return s;
 }
@@ -92,15 +92,15 @@ __device__ __forceinline__ long long seq_units(const Kv4Attend& a, const Seq& s)
     return n;
 }
 
-// U units over `ctas` CTAs: the first U mod G of the G = min(U, ctas) that get
-// work have one unit more than the others.
+// U units over `ctas` CTAs, at least `least` to each: the first U mod G of the G
+// that get work have one unit more than the others.
 struct Shares {
     long long U, q, r;  // q = U / G, r = U mod G
     int G;
     Shares() = default;
-    __device__ __forceinline__ Shares(long long units, int ctas) {
+    __device__ __forceinline__ Shares(long long units, int ctas, int least) {
         U = units;
-        G = (int)min(U, (long long)ctas);
+        G = (int)min(max(U / least, min(U, 1ll)), (long long)ctas);
         if (U < 1ll << 32) {  // a short division
             q = G ? (uint32_t)U / (uint32_t)G : 0;
         } else {
@@ -127,7 +127,7 @@ struct Place {
 // A warp finds CTA `cta`'s share and the tile it begins in (all lanes get it).
 // Lane i holds the lengths of sequence 32 k + i, so up to 32 sequences take one
 // round of loads.  Returns false where the CTA has no work.
-template <int COLS, int UNIT>
+template <int COLS, int UNIT, int LEAST>
 __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas, Shares& sh, Place& p) {
     const int lane = threadIdx.x & 31, hkv = a.pool.kv_heads;
     // sequences b0 + lane, their units, and the units up to and with them (one KV head)
@@ -148,7 +148,7 @@ __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas
         scan(b0);
         total += __shfl_sync(0xffffffffu, incl, 31);
     }
-    sh = Shares(total * hkv, ctas);
+    sh = Shares(total * hkv, ctas, LEAST);
     if (cta >= sh.G) return false;
     const long long u = sh.first(cta);
     long long base = 0;
@@ -177,6 +177,174 @@ __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas
         p.start += n;
     }
     return true;
+}
+
+// The part of a tile that a CTA works on: its units unit0 .. unit1 - 1.
+struct Piece {
+    Place at;
+    KeyRange kr;
+    int unit0, unit1;
+    bool any;  // there is such a piece
+};
+
+template <int COLS, int UNIT>
+__device__ __forceinline__ void cut_piece(const Kv4Attend& a, const Shares& sh, long long from, Piece& p) {
+    p.kr = keys_of<COLS, UNIT>(a, p.at.s, p.at.tile);
+    p.unit0 = (int)(from - p.at.start);
+    p.unit1 = (int)min((long long)p.kr.units, sh.first(blockIdx.x + 1) - p.at.start);
+}
+
+// The piece after p in the CTA's share.
+template <int COLS, int UNIT>
+__device__ __forceinline__ void next_piece(const Kv4Attend& a, const Shares& sh, const Piece& p, Piece& n) {
+    n.any = p.at.start + p.unit1 < sh.first(blockIdx.x + 1);
+    if (!n.any) return;
+    n.at = p.at;
+    n.at.start += p.kr.units;
+    if (++n.at.tile >= n.at.s.tiles) {
+        n.at.tile = 0;
+        if (++n.at.head >= a.pool.kv_heads) {
+            n.at.head = 0;
+            do n.at.s = seq_at<COLS>(a, ++n.at.b);  // (units are left: there is one)
+            while (n.at.s.tiles == 0);
+        }
+    }
+    cut_piece<COLS, UNIT>(a, sh, n.at.start, n);
+}
+
+// Four channels of row n of the sequence, from sums relative to 2^ref.  A row
+// that saw no key (sum 0) is written as zeros, its lse as -infinity.
+template <int D>
+__device__ __forceinline__ void put_row(const Kv4Attend& a, const Seq& s, int kv_head, int n, int d, float4 v, float ref,
+                                        float sum) {
+    const int tok = by_group(a, n), head = kv_head * a.group + n - tok * a.group;
+    const float inv = 1.f / sum;
+    uint2 r = make_uint2(pack_bf16x2(v.x * inv, v.y * inv), pack_bf16x2(v.z * inv, v.w * inv));
+    if (sum == 0.f) r = make_uint2(0u, 0u);
+    *(uint2*)((uint16_t*)a.out.data + (s.row0 + tok) * a.out.st + head * a.out.sh + d) = r;
+    if (a.lse && d == 0)
+        a.lse[(long long)(s.row0 + tok) * a.heads + head] = (ref + log2f(sum)) * 0.6931471805599453f;
+}
+
+// Counts a finished piece of p's tile (the CTA's barrier has ordered its writes
+// before); true where it was the last of CTAs c0 .. c1.  One thread calls it.
+__device__ __forceinline__ bool last_piece(const Kv4Attend& a, int c0, int c1) {
+    // releases the whole CTA's writes, acquires the others'
+    uint32_t n;
+    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(a.done + c0) : "memory");
+    const bool last = n == (uint32_t)(c1 - c0);
+    if (last) a.done[c0] = 0;
+    return last;
+}
+
+// Joins the pieces that CTAs c0 .. c1 left of a tile's `cols` columns from row
+// n0 on; THREADS threads call it and meet at named barrier 1.  D/4 threads hold a column's channels; where columns are few, the
+// pieces of one are shared out among several such teams, which meet in `sm`
+// (32 lanes' part every WARP bytes) and `sm_ml` [THREADS / (D/4)].
+template <int D, int COLS, int THREADS, int WARP>
+__device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int head, int n0, int cols, int c0, int c1,
+                                          uint8_t* sm, float2* sm_ml) {
+    auto sync = [] { named_bar(1, THREADS); };
+    constexpr int LANES = D / 4, TEAMS = THREADS / LANES;
+    const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
+    if (c1 - c0 < 4 && cols > TEAMS) {
+        // few pieces of many columns (a prompt's tile cut at a CTA's border):
+        // four columns a team at a time, their loads all under way together
+        for (int first = team; first < cols; first += 4 * TEAMS) {
+            float2 ml[4][4];
+            float4 y[4][4];
+#pragma unroll
+            for (int k = 0; k < 4; k++)
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const int col = first + k * TEAMS, c = c0 + i;
+                    ml[k][i] = make_float2(-INFINITY, 0.f);
+                    y[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                    if (c <= c1 && col < cols) {
+                        const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
+                        ml[k][i] = __ldcg(&a.part_ml[slot]);
+                        y[k][i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
+                    }
+                }
+#pragma unroll
+            for (int k = 0; k < 4; k++) {
+                if (first + k * TEAMS >= cols) break;
+                const float m = fmaxf(fmaxf(ml[k][0].x, ml[k][1].x), fmaxf(ml[k][2].x, ml[k][3].x));
+                const float ref = m == -INFINITY ? 0.f : m;
+                float sum = 0.f;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    const float f = ex2(ml[k][i].x - ref);
+                    sum = fmaf(f, ml[k][i].y, sum);
+                    v.x = fmaf(f, y[k][i].x, v.x); v.y = fmaf(f, y[k][i].y, v.y);
+                    v.z = fmaf(f, y[k][i].z, v.z); v.w = fmaf(f, y[k][i].w, v.w);
+                }
+                put_row<D>(a, s, head, n0 + first + k * TEAMS, 4 * lane, v, ref, sum);
+            }
+        }
+        sync();
+        return;
+    }
+    int slices = 1;
+    while (2 * slices * cols <= TEAMS) slices *= 2;
+    const int per = TEAMS / slices, slice = team / per;  // columns at a time
+    auto sm_v = [&](int t) { return (float4*)(sm + t * LANES / 32 * WARP) + t * LANES % 32 + lane; };
+    for (int first = 0; first < cols; first += per) {
+        const int col = first + team % per;
+        float m = -INFINITY, sum = 0.f;
+        float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+        // a few pieces at a time, all of their loads under way before the first is used
+        constexpr int AHEAD = 8;
+        for (int b = c0 + slice; b <= c1; b += slices * AHEAD) {
+            float2 ml[AHEAD];
+            float4 y[AHEAD];
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const int c = b + i * slices;
+                ml[i] = make_float2(-INFINITY, 0.f);
+                y[i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                if (c <= c1 && col < cols) {
+                    const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
+                    ml[i] = __ldcg(&a.part_ml[slot]);
+                    y[i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
+                }
+            }
+            const float old = m;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) m = fmaxf(m, ml[i].x);
+            const float ref = m == -INFINITY ? 0.f : m, f0 = ex2(old - ref);
+            sum *= f0;
+            v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
+#pragma unroll
+            for (int i = 0; i < AHEAD; i++) {
+                const float f = ex2(ml[i].x - ref);
+                sum = fmaf(f, ml[i].y, sum);
+                v.x = fmaf(f, y[i].x, v.x); v.y = fmaf(f, y[i].y, v.y);
+                v.z = fmaf(f, y[i].z, v.z); v.w = fmaf(f, y[i].w, v.w);
+            }
+        }
+        *sm_v(team) = v;
+        if (lane == 0) sm_ml[team] = make_float2(m, sum);
+        sync();
+        if (slice == 0 && col < cols) {
+            float mm = -INFINITY;
+            for (int i = 0; i < slices; i++) mm = fmaxf(mm, sm_ml[team + i * per].x);
+            const float ref = mm == -INFINITY ? 0.f : mm;
+            sum = 0.f;
+            v = make_float4(0.f, 0.f, 0.f, 0.f);
+            for (int i = 0; i < slices; i++) {
+                const float2 ml = sm_ml[team + i * per];
+                const float4 y = *sm_v(team + i * per);
+                const float f = ex2(ml.x - ref);
+                sum = fmaf(f, ml.y, sum);
+                v.x = fmaf(f, y.x, v.x); v.y = fmaf(f, y.y, v.y);
+                v.z = fmaf(f, y.z, v.z); v.w = fmaf(f, y.w, v.w);
+            }
+            put_row<D>(a, s, head, n0 + col, 4 * lane, v, ref, sum);
+        }
+        sync();
+    }
 }
 
 }  // namespace sp

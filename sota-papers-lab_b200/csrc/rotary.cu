@@ -29,7 +29,7 @@ __global__ void __launch_bounds__(256) sp_rope(const Rows x, const Rows out, con
     const Unit un = unit_at(u, r);
     const int pos = r.positions[t];
     if (pos < 0 || pos >= r.limit) {  // the row is left as it was
-        if (lane == 0) atomicOr(err, ERR_INDEX);
+        if (lane == 0) atomicOr(err + ERR_INDEX_WORD, ERR_INDEX);
         return;
     }
     Chunk<DT> lo[HPT], hi[HPT];

@@ -18,7 +18,10 @@ namespace sp {
 
 // Bit of the device error word: an index read from device memory (a
 // position, slot, page or length) was out of range (SPL_SAGE_DEVERR_INDEX).
+// In the word beside the one that the kernels' waits look at: a wait gives up
+// when another kernel's wait has, but not because of an index.
 constexpr uint32_t ERR_INDEX = 1u << 2;
+constexpr int ERR_INDEX_WORD = 1;
 
 struct Unit {
     int c0, c1;  // first channel of each chunk

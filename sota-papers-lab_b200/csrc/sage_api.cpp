@@ -909,13 +909,17 @@ int spl_sage_quantize_noalloc(void* stream, int head_dim, int pv_accum, const sp
 
 int spl_sage_engine_status(spl_sage* s, uint32_t* device_error_word) {
     if (!s) return fail(SPL_SAGE_ERR_INVALID, "spl_sage_engine_status: NULL argument");
-    uint32_t w = 0;
-    cudaError_t e = cudaMemcpyAsync(&w, s->err, 4, cudaMemcpyDeviceToHost, s->stream);
+    uint32_t two[2] = {0, 0};  // the waits' word, and that of the indices in device memory
+    cudaError_t e = cudaMemcpyAsync(two, s->err, 8, cudaMemcpyDeviceToHost, s->stream);
     if (e == cudaSuccess) e = cudaStreamSynchronize(s->stream);
     if (e != cudaSuccess) return cuda_fail(e, "read engine status");
+    const uint32_t w = two[0] | two[1];
     if (device_error_word) *device_error_word = w;
     if (w) {
-        cudaMemsetAsync(s->err, 0, 4, s->stream);
+        cudaMemsetAsync(s->err, 0, 8, s->stream);
+        if (!two[0])
+            return fail(SPL_SAGE_ERR_KERNEL,
+                        "a kernel met a position, slot, page id or length out of range (device error word 0x%08x)", w);
         return fail(SPL_SAGE_ERR_KERNEL, "kernel reported device error word 0x%08x (timeout site %u)", w,
                     (w >> 8) & 0xff);
     }

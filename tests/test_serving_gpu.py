@@ -352,8 +352,8 @@ class Batch:
                 continue
             p = self.pages[b, :-(-n // self.page)].long()
             k, v = (x[p].transpose(1, 2).reshape(-1, hkv, d)[:n] for x in (kh, vh))
-            # a probability times its V scale is rounded to bf16, by at most 2^-8; it weighs n - 8
-            w = (vn[p].transpose(1, 2).reshape(-1, hkv, d)[:n] - 8).abs() * vs[p].transpose(1, 2).reshape(
+            # a probability times its V scale is rounded to f16, by at most 2^-11; it weighs n
+            w = vn[p].transpose(1, 2).reshape(-1, hkv, d)[:n] * vs[p].transpose(1, 2).reshape(
                 -1, hkv, d // 64)[:n].repeat_interleave(64, -1)
             j = torch.arange(n, device=DEV)
             at = n - qn + torch.arange(qn, device=DEV)[:, None]
@@ -373,8 +373,10 @@ class Batch:
                 pr = torch.where(see[:, None], torch.exp(x - torch.where(lse == -math.inf, 0.0, lse)[..., None]), 0.0)
                 o = torch.einsum("tgk,kd->tgd", pr, v[:, h])
                 off = 24 * 2.0 ** -24 * size + 2.0 ** -20
-                tol = (2.0 ** -8 * o.abs() + 2.0 ** -8 * torch.einsum("tgk,kd->tgd", pr, w[:, h])
+                tol = (2.0 ** -8 * o.abs() + 2.0 ** -11 * torch.einsum("tgk,kd->tgd", pr, w[:, h])
                        + (2 * off[..., None]) * (v[:, h].abs().amax() if n else 0.0) + 1e-30)
+                if max(self.qn) * g > 128:  # many rows: V's values and the probabilities are rounded to f16 (2^-11)
+                    tol = tol + 2 * 2.0 ** -11 * torch.einsum("tgk,kd->tgd", pr, v[:, h].abs())
                 got = self.out[row:row + qn, h * g:(h + 1) * g].double()
                 bad = (got - o).abs() > tol
                 assert not bad.any(), (what, b, h, bad.nonzero()[:4].tolist(), (got - o).abs().max().item())
@@ -464,11 +466,11 @@ def test_attend_strided_rows(engines):
     b.check()
 
 
-@pytest.mark.parametrize("rows", [1, 4, 40])
+@pytest.mark.parametrize("rows", [1, 4, 40, 90])
 def test_attend_nan_reaches_only_the_rows_that_see_it(engines, rows):
     """A cached NaN (K of one token, V of one group of another) spreads to
     the queries that see it and to no other; a V group's only to its channels."""
-    d, eng, n = 128, engines[128], 100
+    d, eng, n = 128, engines[128], 300
     for part in ("k", "v"):
         b = Batch(d, 16, 2, 1, [n], [rows], tail_rows=0)
         at = n - rows + rows // 2  # seen by the later half of the queries
