@@ -639,25 +639,22 @@ class SageAttention:
 
     def _rows(self, what: str, t, dtypes, tokens: int, heads: int) -> _Tensor:
         """A CUDA tensor [tokens][heads][head_dim] of this engine's device as a view."""
-        st = t.stride()
-        if not t.is_cuda or t.device.index != self.device or t.dtype not in dtypes:
+        shape, st = t.shape, t.stride()
+        if t.get_device() != self.device or t.dtype not in dtypes:
             raise SageError(ERR_INVALID, f"{what} must be a tensor of {' or '.join(str(x) for x in dtypes)} on device "
                                          f"{self.device}, got {t.dtype} on {t.device}")
-        if tuple(t.shape) != (tokens, heads, self.head_dim) or (st[2] != 1 and t.numel()):
+        empty = tokens == 0 or heads == 0
+        if shape != (tokens, heads, self.head_dim) or (st[2] != 1 and not empty):
             raise SageError(ERR_INVALID, f"{what} must be [{tokens}][{heads}][{self.head_dim}] with channels "
-                                         f"contiguous, got {tuple(t.shape)} with strides {st}")
-        if min(st) < 0:
-            raise SageError(ERR_INVALID, f"{what} has a negative stride")
+                                         f"contiguous, got {tuple(shape)} with strides {st}")
         # a stride of an axis of length 1 is never used
         a = st[0] if tokens > 1 else 0
         b = st[1] if heads > 1 else 0
-        return _Tensor(t.data_ptr(), (tokens - 1) * a + (heads - 1) * b + self.head_dim if t.numel() else 0, 0, a, b)
+        return _Tensor(t.data_ptr(), 0 if empty else (tokens - 1) * a + (heads - 1) * b + self.head_dim, 0, a, b)
 
     def _index(self, what: str, t, shape: tuple) -> int:
         """The address of an int32 CUDA array of this engine's device."""
-        import torch
-        if (not t.is_cuda or t.device.index != self.device or t.dtype != torch.int32 or tuple(t.shape) != shape
-                or not t.is_contiguous()):
+        if t.get_device() != self.device or t.dtype != _torch().int32 or t.shape != shape or not t.is_contiguous():
             raise SageError(ERR_INVALID, f"{what} must be a contiguous int32 tensor {list(shape)} on device "
                                          f"{self.device}, got {t.dtype} {list(t.shape)} on {t.device}")
         return t.data_ptr()
@@ -666,10 +663,12 @@ class SageAttention:
         """out = R(positions) x for x [tokens][heads][head_dim] in bf16, f16 or
         f32 (spl_sage_rope); out of the same shape and type may be x.
         backward: the transposed rotation, the gradient's."""
-        types = _rope_types()
-        t, h = x.shape[0], x.shape[1]
-        cx, co = self._rows("x", x, tuple(types), t, h), self._rows("output", out, (x.dtype,), t, h)
-        _check(lib().spl_sage_rope(self._h, types[x.dtype], t, h, cx, co, ctypes.byref(rotary._c(self)),
+        _torch()
+        if x.dim() != 3:
+            raise SageError(ERR_INVALID, f"x must be [tokens][heads][{self.head_dim}], got {list(x.shape)}")
+        t, h, _ = x.shape
+        cx, co = self._rows("x", x, _ROPE_TYPES, t, h), self._rows("output", out, (x.dtype,), t, h)
+        _check(lib().spl_sage_rope(self._h, _ROPE_TYPES[x.dtype], t, h, cx, co, ctypes.byref(rotary._c(self)),
                                    self._index("positions", positions, (t,)), int(backward)))
 
     def kv4_append(self, cache: "Kv4Cache", k, v, slots, *, rotary: "Rotary | None" = None, positions=None, q=None,
@@ -678,8 +677,8 @@ class SageAttention:
         [tokens][kv_heads][head_dim] at slots (int32 [tokens], -1: not
         cached), K rotated by positions where a rotary is given; q bf16
         [tokens][heads][head_dim] is rotated into q_out on the way."""
-        import torch
-        bf, t, c = (torch.bfloat16,), k.shape[0], cache._c(self)
+        _torch()
+        bf, t, c = _BF16, k.shape[0], cache._c(self)
         ck, cv = self._rows("K", k, bf, t, c.kv_heads), self._rows("V", v, bf, t, c.kv_heads)
         if (q is None) != (q_out is None):
             raise SageError(ERR_INVALID, "Q and its output are given together, or neither")
@@ -696,8 +695,8 @@ class SageAttention:
     def kv4_read(self, cache: "Kv4Cache", slots, k, v):
         """The cached values at slots into k and v, bf16
         [tokens][kv_heads][head_dim] (spl_sage_kv4_read)."""
-        import torch
-        bf, t, c = (torch.bfloat16,), slots.shape[0], cache._c(self)
+        _torch()
+        bf, t, c = _BF16, slots.shape[0], cache._c(self)
         ck, cv = self._rows("K", k, bf, t, c.kv_heads), self._rows("V", v, bf, t, c.kv_heads)
         _check(lib().spl_sage_kv4_read(self._h, ctypes.byref(c), t, self._index("slots", slots, (t,)), ck, cv))
 
@@ -712,11 +711,11 @@ class SageAttention:
         [batch], q_start int32 [batch + 1] (None: one query per sequence), at
         most max_q queries a sequence; writes out and, where given, lse f32
         [tokens][heads]."""
-        import torch
-        bf, t, h, c, b = (torch.bfloat16,), q.shape[0], q.shape[1], cache._c(self), kv_len.shape[0]
+        torch = _torch()
+        bf, t, h, c, b = _BF16, q.shape[0], q.shape[1], cache._c(self), kv_len.shape[0]
         cq, co = self._rows("Q", q, bf, t, h), self._rows("output", out, bf, t, h)
-        if lse is not None and (not lse.is_cuda or lse.device.index != self.device or lse.dtype != torch.float32
-                                or tuple(lse.shape) != (t, h) or not lse.is_contiguous()):
+        if lse is not None and (lse.get_device() != self.device or lse.dtype != torch.float32 or lse.shape != (t, h)
+                                or not lse.is_contiguous()):
             raise SageError(ERR_INVALID, f"lse must be a contiguous f32 tensor [{t}][{h}] on device {self.device}")
         if pages.dim() != 2:
             raise SageError(ERR_INVALID, f"pages must be [batch][max_pages], got {list(pages.shape)}")
@@ -939,16 +938,20 @@ class RopeTable:
         return cls(RopeLayout.one_d(head_dim), rope_table_1d(base, head_dim, positions))
 
 
-_ROPE_TYPES = None
+_TORCH = None
+_ROPE_TYPES: dict = {}  # torch types of SageAttention.rope -> SPL_SAGE_BF16, _F16, _F32
+_BF16: tuple = ()
 
 
-def _rope_types() -> dict:
-    """torch types of SageAttention.rope -> SPL_SAGE_BF16, _F16, _F32."""
-    global _ROPE_TYPES
-    if _ROPE_TYPES is None:
+def _torch():
+    """torch, imported by the first call that takes tensors."""
+    global _TORCH, _BF16
+    if _TORCH is None:
         import torch
-        _ROPE_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
-    return _ROPE_TYPES
+        _ROPE_TYPES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
+        _BF16 = (torch.bfloat16,)
+        _TORCH = torch
+    return _TORCH
 
 
 @dataclass(frozen=True)
@@ -1000,18 +1003,21 @@ class Rotary:
     (2p, 2p + 1) where interleaved (spl_sage_rotary)."""
 
     def __init__(self, table, rot_dim: int, interleaved: bool = False):
-        import torch
-        if (not table.is_cuda or table.dtype != torch.float32 or not table.is_contiguous() or table.dim() != 3
-                or tuple(table.shape[1:]) != (rot_dim // 2, 2)):
+        shape = table.shape
+        if (not table.is_cuda or table.dtype != _torch().float32 or not table.is_contiguous() or len(shape) != 3
+                or shape[1] != rot_dim // 2 or shape[2] != 2):
             raise SageError(ERR_INVALID, f"a rotary table is a contiguous f32 CUDA tensor [positions][{rot_dim // 2}]"
                                          f"[2], got {table.dtype} {list(table.shape)} on {table.device}")
         self.table, self.rot_dim, self.interleaved = table, rot_dim, interleaved
-        self._struct = _Rotary(table.data_ptr(), table.shape[0], rot_dim, int(interleaved))
+        self._struct = _Rotary(table.data_ptr(), shape[0], rot_dim, int(interleaved))
 
     def _c(self, eng: "SageAttention") -> _Rotary:
-        if self.table.device.index != eng.device:
+        if self.table.get_device() != eng.device:
             raise SageError(ERR_INVALID, f"the rotary table is on {self.table.device}, the engine on device {eng.device}")
         return self._struct
+
+
+_KV4_BLOCKS: dict = {}  # (head dim, page tokens) -> bytes of a block
 
 
 class Kv4Cache:
@@ -1020,23 +1026,24 @@ class Kv4Cache:
     contiguous; a view of every second page, say, is fine."""
 
     def __init__(self, pool, page_tokens: int, head_dim: int):
-        import torch
         block = Kv4Cache.block_bytes(head_dim, page_tokens)
-        st = pool.stride()
-        if (not pool.is_cuda or pool.dtype != torch.uint8 or pool.dim() != 3 or pool.shape[2] != block or st[2] != 1
-                or (pool.shape[1] > 1 and st[1] != block)):
+        shape, st = pool.shape, pool.stride()
+        if (not pool.is_cuda or pool.dtype != _torch().uint8 or len(shape) != 3 or shape[2] != block or st[2] != 1
+                or (shape[1] > 1 and st[1] != block)):
             raise SageError(ERR_INVALID, f"a cache pool is a uint8 CUDA tensor [pages][kv_heads][{block}] with "
                                          f"contiguous pages, got {pool.dtype} {list(pool.shape)} with strides {st} on "
                                          f"{pool.device}")
         self.pool, self.page_tokens, self.head_dim = pool, page_tokens, head_dim
-        pages, heads = pool.shape[0], pool.shape[1]
+        pages, heads = shape[0], shape[1]
         stride = st[0] if pages > 1 else heads * block
         self._struct = _Kv4(pool.data_ptr(), pages, stride, page_tokens, heads)
 
     @staticmethod
     def block_bytes(head_dim: int, page_tokens: int) -> int:
         """Bytes of one page of one KV head."""
-        n = lib().spl_sage_kv4_block_bytes(head_dim, page_tokens)
+        n = _KV4_BLOCKS.get((head_dim, page_tokens))
+        if n is None:
+            n = _KV4_BLOCKS[head_dim, page_tokens] = lib().spl_sage_kv4_block_bytes(head_dim, page_tokens)
         if not n:
             raise SageError(ERR_INVALID, f"no 4-bit cache for head dim {head_dim} and pages of {page_tokens} tokens: "
                                          "64 or 128, and 16, 32, 64 or 128")
@@ -1050,7 +1057,7 @@ class Kv4Cache:
         return Kv4Cache(torch.zeros(pages, kv_heads, block, dtype=torch.uint8, device="cuda"), page_tokens, head_dim)
 
     def _c(self, eng: "SageAttention") -> _Kv4:
-        if self.head_dim != eng.head_dim or self.pool.device.index != eng.device:
+        if self.head_dim != eng.head_dim or self.pool.get_device() != eng.device:
             raise SageError(ERR_INVALID, f"the cache is for head dim {self.head_dim} on {self.pool.device}, the engine "
                                          f"for {eng.head_dim} on device {eng.device}")
         return self._struct

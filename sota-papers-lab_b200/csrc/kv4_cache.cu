@@ -22,18 +22,26 @@ namespace sp {
 
 constexpr float FINITE_MAX = 3.402823466e38f;
 
-// One 8-channel chunk's minimum and maximum; a NaN or an infinity makes the
-// range infinite, which marks the group.
+// Minimum and maximum that a NaN gets through.
+__device__ __forceinline__ float min_nan(float a, float b) {
+    float d;
+    asm("min.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+__device__ __forceinline__ float max_nan(float a, float b) {
+    float d;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+    return d;
+}
+
+// One 8-channel chunk's minimum and maximum.
 __device__ __forceinline__ void chunk_range(const float (&x)[8], float& mn, float& mx) {
     mn = mx = x[0];
-    bool fine = true;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        mn = fminf(mn, x[i]);
-        mx = fmaxf(mx, x[i]);
-        fine = fine && fabsf(x[i]) <= FINITE_MAX;
+    for (int i = 1; i < 8; i++) {
+        mn = min_nan(mn, x[i]);
+        mx = max_nan(mx, x[i]);
     }
-    if (!fine) mn = -INFINITY;
 }
 
 // Scale and zero of a group (bf16 bits, scale in the low half) and what the
@@ -66,18 +74,33 @@ __device__ __forceinline__ GroupScale group_scale(float mn, float mx) {
 // n of 8 channels, channel i at bits 4i.  (x - zero) / scale is the product
 // with the reciprocal corrected once by its exact remainder (Markstein: the
 // quotient rounded to nearest, given a correctly rounded reciprocal); ties of
-// the quotient, common for bf16 inputs, come out as ties.
+// the quotient, common for bf16 inputs, come out as ties.  Adding 1.5 * 2^23
+// rounds to the nearest even integer and leaves it in the low bits; the eight
+// are put together by Horner's rule in 32-bit arithmetic, in which the
+// constant's bits add up to another constant.
 __device__ __forceinline__ uint32_t quantise8(const float (&x)[8], const GroupScale& g) {
+    constexpr uint32_t BITS = 0x4b400000u;  // of 1.5 * 2^23
+    auto mul2 = [](uint64_t a, uint64_t b) {  // (its result is only ever multiplied or added to: nothing to fuse it with)
+        uint64_t d;
+        asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+        return d;
+    };
+    const uint64_t zero = pk2(g.zero, g.zero), less = pk2(-g.scale, -g.scale), inv = pk2(g.inv, g.inv);
     uint32_t w = 0;
 #pragma unroll
-    for (int i = 0; i < 8; i++) {
-        const float y = __fsub_rn(x[i], g.zero);
-        float q = __fmul_rn(y, g.inv);
-        q = __fmaf_rn(__fmaf_rn(-q, g.scale, y), g.inv, q);
-        const int n = __float2int_rn(fminf(fmaxf(q, 0.f), 15.f));
-        w |= (uint32_t)n << (4 * i);
+    for (int i = 6; i >= 0; i -= 2) {
+        const uint64_t y = sub2(pk2(x[i], x[i + 1]), zero);
+        uint64_t q = mul2(y, inv);
+        q = fma2(fma2(q, less, y), inv, q);
+        float q0, q1;
+        upk2(q, q0, q1);
+        q0 = fminf(fmaxf(q0, 0.f), 15.f);  // (a NaN: 0)
+        q1 = fminf(fmaxf(q1, 0.f), 15.f);
+        upk2(add2(pk2(q0, q1), pk2(12582912.f, 12582912.f)), q0, q1);
+        w = w * 16u + __float_as_uint(q1);
+        w = w * 16u + __float_as_uint(q0);
     }
-    return w;
+    return w - BITS * 0x11111111u;
 }
 
 template <int D, int HPT>
@@ -151,12 +174,12 @@ __global__ void __launch_bounds__(256) sp_kv4_append(const Kv4Pool pool, const R
 #pragma unroll
         for (int j = 0; j < NG; j++) {
             const bool ia = x.c0 / KV4_GROUP == j, ib = x.c1 / KV4_GROUP == j;
-            float mn = fminf(ia ? amn : INFINITY, ib ? bmn : INFINITY);
-            float mx = fmaxf(ia ? amx : -INFINITY, ib ? bmx : -INFINITY);
+            float mn = min_nan(ia ? amn : INFINITY, ib ? bmn : INFINITY);
+            float mx = max_nan(ia ? amx : -INFINITY, ib ? bmx : -INFINITY);
 #pragma unroll
             for (int m = 1; m < UNITS; m *= 2) {
-                mn = fminf(mn, __shfl_xor_sync(0xffffffffu, mn, m));
-                mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, m));
+                mn = min_nan(mn, __shfl_xor_sync(0xffffffffu, mn, m));
+                mx = max_nan(mx, __shfl_xor_sync(0xffffffffu, mx, m));
             }
             g[j] = group_scale(mn, mx);
         }
@@ -179,11 +202,15 @@ static cudaError_t append(const Kv4Pool& pool, const Rows& q, const Rows& q_out,
                           cudaStream_t st) {
     constexpr int HL = 512 / D;
     const int rows = q_heads + 2 * pool.kv_heads;
-    // Four rows a thread once that still leaves every SM a few warps.
-    const bool many = (long long)tokens * ((rows + 4 * HL - 1) / (4 * HL)) >= 148 * 16;
-    const int per = many ? 4 : 1, rb = (rows + per * HL - 1) / (per * HL);
+    // Two rows a thread once that still leaves every SM a few warps (append and
+    // read back of 8192 tokens, 32 / 8 heads, D = 128: 62 us, with 1 66, with 4
+    // 70, whose registers leave two blocks on an SM; 1370 tokens of 16 heads, D
+    // = 64: 9.1, 8.9, 10.7).
+    constexpr int MANY = 2;
+    const bool many = (long long)tokens * ((rows + MANY * HL - 1) / (MANY * HL)) >= 148 * 16;
+    const int per = many ? MANY : 1, rb = (rows + per * HL - 1) / (per * HL);
     const unsigned grid = (unsigned)(((long long)tokens * rb + 7) / 8);
-    return launch_after_previous(many ? sp_kv4_append<D, 4> : sp_kv4_append<D, 1>, dim3(grid), dim3(256), 0, st, pool, q,
+    return launch_after_previous(many ? sp_kv4_append<D, MANY> : sp_kv4_append<D, 1>, dim3(grid), dim3(256), 0, st, pool, q,
                                  q_out, k, v, r, slots, tokens, q_heads, rb, err);
 }
 
@@ -195,52 +222,63 @@ cudaError_t launch_kv4_append(int d, const Kv4Pool& pool, const Rows& q, const R
 }
 
 // The values at given slots, zero + scale * n rounded once to bf16.  A thread
-// reads one word (8 channels) and writes 16 bytes; bound by the bf16 rows it
-// writes.
+// reads one word (8 channels) of READ_TOKENS tokens and writes 16 bytes of
+// each; bound by the bf16 rows it writes.
+constexpr int READ_TOKENS = 4;
+
 template <int D>
 __global__ void __launch_bounds__(256) sp_kv4_read(const Kv4Pool pool, const int* __restrict__ slots, const Rows k,
                                                    const Rows v, int tokens, uint32_t* __restrict__ err) {
     constexpr int CH = D / 8, NG = D / KV4_GROUP;
     griddep_wait();
     griddep_launch_dependents();
-    const long long i = (long long)blockIdx.x * blockDim.x + threadIdx.x;
-    const int c = (int)(i % CH);
-    const long long rowi = i / CH;
-    const int rows = 2 * pool.kv_heads;
-    const int row = (int)(rowi % rows);
-    const long long t = rowi / rows;
-    if (t >= tokens) return;
-    const int slot = slots[t];
-    const int page = slot >> pool.page_shift;
-    if (page >= pool.pages) {
-        if (c == 0 && row == 0) atomicOr(err + ERR_INDEX_WORD, ERR_INDEX);
-        return;
-    }
+    const int c = threadIdx.x % CH, row = blockIdx.y * (256 / CH) + threadIdx.x / CH;
+    if (row >= 2 * pool.kv_heads) return;
     const bool is_v = row >= pool.kv_heads;
-    const int h = is_v ? row - pool.kv_heads : row;
-    const Rows& dst = is_v ? v : k;
-    float f[8] = {};
-    if (slot >= 0) {
-        const int in_page = slot & (pool.page_tokens - 1);
-        const uint8_t* blk = pool.data + page * pool.page_stride + (long long)h * pool.block;
-        const int half = pool.page_tokens * (D / 2), par = pool.page_tokens * NG * 4;
-        const uint32_t w = *(const uint32_t*)(blk + (is_v ? half : 0) + in_page * (D / 2) + c * 4);
-        const uint32_t p = ((const uint32_t*)(blk + 2 * half + (is_v ? par : 0)))[in_page * NG + c * 8 / KV4_GROUP];
-        const float scale = __uint_as_float(p << 16), zero = __uint_as_float(p & 0xffff0000u);
+    const int h = is_v ? row - pool.kv_heads : row, t0 = blockIdx.x * READ_TOKENS;
+    const int half = pool.page_tokens * (D / 2), par = pool.page_tokens * NG * 4;
+    const uint8_t* head = pool.data + (long long)h * pool.block;
+    uint32_t w[READ_TOKENS], p[READ_TOKENS];
+    bool put[READ_TOKENS];
 #pragma unroll
-        for (int j = 0; j < 8; j++) f[j] = __fmaf_rn(scale, (float)((w >> (4 * j)) & 15u), zero);
+    for (int i = 0; i < READ_TOKENS; i++) {
+        w[i] = p[i] = 0;
+        put[i] = t0 + i < tokens;
+        if (!put[i]) continue;
+        const int slot = slots[t0 + i], page = slot >> pool.page_shift;
+        if (page >= pool.pages) {
+            if (c == 0 && row == 0) atomicOr(err + ERR_INDEX_WORD, ERR_INDEX);
+            put[i] = false;
+        } else if (slot >= 0) {
+            const int in_page = slot & (pool.page_tokens - 1);
+            const uint8_t* blk = head + page * pool.page_stride;
+            w[i] = *(const uint32_t*)(blk + (is_v ? half : 0) + in_page * (D / 2) + c * 4);
+            p[i] = ((const uint32_t*)(blk + 2 * half + (is_v ? par : 0)))[in_page * NG + c * 8 / KV4_GROUP];
+        }
     }
-    Chunk<0> o;
-    o.from(f);
-    o.store((void*)dst.data, t * dst.st + h * dst.sh + 8 * c);
+    const Rows& dst = is_v ? v : k;
+#pragma unroll
+    for (int i = 0; i < READ_TOKENS; i++) {
+        if (!put[i]) continue;
+        const float scale = __uint_as_float(p[i] << 16), zero = __uint_as_float(p[i] & 0xffff0000u);
+        float f[8];
+#pragma unroll
+        for (int j = 0; j < 8; j++) {
+            const float n = __uint_as_float(((w[i] >> (4 * j)) & 15u) | 0x4b000000u) - 8388608.f;  // 2^23 + n, n
+            f[j] = __fmaf_rn(scale, n, zero);
+        }
+        Chunk<0> o;
+        o.from(f);
+        o.store((void*)dst.data, (t0 + i) * dst.st + h * dst.sh + 8 * c);
+    }
 }
 
 cudaError_t launch_kv4_read(int d, const Kv4Pool& pool, const int* slots, const Rows& k, const Rows& v, int tokens,
                             uint32_t* err, cudaStream_t st) {
-    const long long n = (long long)tokens * 2 * pool.kv_heads * (d / 8);
-    const unsigned grid = (unsigned)((n + 255) / 256);
-    return launch_after_previous(d == 64 ? sp_kv4_read<64> : sp_kv4_read<128>, dim3(grid), dim3(256), 0, st, pool, slots,
-                                 k, v, tokens, err);
+    const int rows_a_block = 256 / (d / 8);
+    const dim3 grid((tokens + READ_TOKENS - 1) / READ_TOKENS, (2 * pool.kv_heads + rows_a_block - 1) / rows_a_block);
+    return launch_after_previous(d == 64 ? sp_kv4_read<64> : sp_kv4_read<128>, grid, dim3(256), 0, st, pool, slots, k, v,
+                                 tokens, err);
 }
 
 }  // namespace sp

@@ -50,8 +50,9 @@ __device__ __forceinline__ void load_angles(const RotaryArgs& r, int position, i
 // y = (a c - b s, b c + a s) on the unit's 16 channels (lo, hi: its chunks).
 // Every product and sum is rounded on its own: no fused multiply-add, so that
 // the same formula written with separate operations gives the same bits (the
-// 4-bit values that follow depend on them).  `back`: the transposed rotation
-// (the gradient), s with the other sign.
+// 4-bit values that follow depend on them).  (Not as packed f32x2 products and
+// sums, which are fused all the same.)  `back`: the transposed rotation (the
+// gradient), s with the other sign.
 __device__ __forceinline__ void turn(float (&lo)[8], float (&hi)[8], const float (&cs)[16], bool interleaved,
                                      bool back) {
 #pragma unroll
