@@ -289,8 +289,11 @@ int spl_sage_kv4_ws_create(spl_sage* s, spl_sage_kv4_ws** out) {
     ws->head_dim = s->head_dim;
     ws->bytes = sp::kv4_scratch_bytes(s->head_dim, s->sm_count);
     cudaError_t e = cudaMalloc(&ws->mem, ws->bytes);
-    if (e == cudaSuccess && (e = cudaMemsetAsync(ws->mem, 0, sp::KV4_COUNTS, s->stream)) != cudaSuccess)
-        cudaFree(ws->mem);
+    if (e == cudaSuccess) {
+        e = cudaMemsetAsync(ws->mem, 0, sp::KV4_COUNTS, s->stream);
+        if (e == cudaSuccess) e = cudaStreamSynchronize(s->stream);  // another engine's stream may use it first
+        if (e != cudaSuccess) cudaFree(ws->mem);
+    }
     if (e != cudaSuccess) {
         delete ws;
         return cuda_fail(e, "allocate the cache attention's workspace");

@@ -178,7 +178,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
     if (tid == 0) sm_gave_up = 0;
 
     griddep_wait();
-    griddep_launch_dependents();
     if (blockIdx.x == 0)  // what is out of range is reported once
         for (int b = tid; b < a.batch; b += PR_THREADS) seq_at<PR_ROWS>(a, b, true);
     if (warp == 0) {
@@ -218,6 +217,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
         tmem_alloc(smem_u32(&tmem_base_s), 512);
         tmem_relinquish();
     }
+    // (not before TMEM is taken: a kernel that starts early may take it for itself and wait for this one)
+    griddep_launch_dependents();
     fence_proxy_async_smem();
     tc_fence_before();
     __syncthreads();
@@ -239,9 +240,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             const int n = p.unit1 - p.unit0, n0 = p.at.tile * PR_ROWS, rows = s.qn * a.group;
             const bool two = n0 + 128 < rows;  // B has rows
             const int nr = n0 + x * 128 + row;
-            // ---- the row of Q, scaled by the power of two that brings the
-            // piece's largest magnitude to [2^13, 2^14), channels of each 8 in
-            // the order 0 4 1 5 2 6 3 7 (that of K's nibbles)
+            // ---- the rows of Q, scaled by the power of two that brings the
+            // piece's largest finite magnitude to [2^13, 2^14) (bf16 values
+            // down to 2^-28 of it stay exact; what is not finite stays in its
+            // own row), channels of each 8 in the order 0 4 1 5 2 6 3 7 (that
+            // of K's nibbles)
             {
                 // D/8 lanes hold a row's 16-byte pieces: 256/D rows of the warp's 32 at a time
                 constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, TURNS = 32 / AT_ONCE;
@@ -261,7 +264,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     float f[8];
                     unpack_bf16x8(w[i], f);
 #pragma unroll
-                    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(f[j]));
+                    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
                 }
                 amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
                 if (lane == 0) sm_amax[warp] = amax;

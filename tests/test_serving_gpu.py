@@ -486,6 +486,63 @@ def test_attend_nan_reaches_only_the_rows_that_see_it(engines, rows):
     eng.engine_status()
 
 
+@pytest.mark.parametrize("rows", [1, 4, 90])
+def test_attend_query_that_is_not_finite_stays_in_its_row(engines, rows):
+    d, eng = 128, engines[128]
+    b = Batch(d, 16, 4, 2, [300], [rows], tail_rows=0)
+    b.fill(eng)
+    b.attend(eng, engines["ws", d])
+    right = b.out.clone()
+    b.q[0, 0, 5], b.q[rows // 2, 1, 77], b.q[rows - 1, 3, 0] = math.nan, math.inf, -math.inf
+    b.attend(eng, engines["ws", d])
+    hit = torch.zeros(rows, 4, dtype=torch.bool, device=DEV)
+    hit[0, 0] = hit[rows // 2, 1] = hit[rows - 1, 3] = True
+    assert torch.equal(b.out[~hit], right[~hit]) and torch.isnan(b.out[hit]).any(-1).all()
+    eng.engine_status()
+
+
+@pytest.mark.parametrize("rows", [1, 9, 150])
+@pytest.mark.parametrize("d", [64, 128])
+def test_attend_uneven_magnitudes(engines, d, rows):
+    """Keys 50 and values 500 times as large as their neighbours', query rows
+    a thousandth of the others', constant groups."""
+    eng = engines[d]
+    b = Batch(d, 32, 4, 2, [700], [rows], seed=rows + d, tail_rows=0)
+    b.k[::97] *= 50
+    b.v[5::89] *= 500
+    b.v[3::50] = 0.75
+    b.k[9::70] = 0.0
+    b.q[::3] *= 1e-3
+    b.fill(eng)
+    b.attend(eng, engines["ws", d])
+    b.check()
+
+
+def test_index_errors_leave_other_kernels_alone(engines):
+    """A bad slot sets the index bit; the projection and attention that follow
+    on the same engine (whose waits look at the error word) run all the same."""
+    eng, d = engines[128], 128
+    g = gen(4)
+    cache = sage.Kv4Cache.empty(2, 2, 16, d)
+    x = rand(g, 1, 2, d)
+    h = rand(g, 256, 512)
+    w = rand(g, (4 + 2 + 2) * d, 512)
+    q = torch.zeros(256, 4, d, dtype=torch.bfloat16, device=DEV)
+    k, v = (torch.zeros(256, 2, d, dtype=torch.bfloat16, device=DEV) for _ in range(2))
+    q2 = q.clone()
+    eng.qkv_gemm(h, w, None, None, q2, k, v, batch=1, tokens=256, heads=4, kv_heads=2)
+    eng.kv4_append(cache, x, x, ints([99]))
+    eng.qkv_gemm(h, w, None, None, q, k, v, batch=1, tokens=256, heads=4, kv_heads=2)
+    b = Batch(d, 16, 4, 2, [300], [90], tail_rows=0)
+    b.fill(eng)
+    b.attend(eng, engines["ws", d])
+    b.check()
+    assert torch.equal(q, q2)
+    with pytest.raises(sage.SageError, match="out of range"):
+        eng.engine_status()
+    eng.engine_status()
+
+
 def test_attend_bad_indices_are_reported(engines):
     """Wild page ids, lengths and q_start stay inside the buffers, set the
     error word, and leave the other sequences right."""
