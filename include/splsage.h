@@ -561,9 +561,11 @@ int spl_sage_kv4_read(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, co
                       spl_sage_tensor_mut k, spl_sage_tensor_mut v);
 
 /* Scratch of spl_sage_kv4_attend (partial outputs of sequences that are split
- * over the GPU), for any shape on this engine's GPU and head dim.  Calls that
- * share one must not run at the same time: use one per stream, and one per
- * captured graph if graphs are replayed side by side. */
+ * over the GPU), for any shape on this engine's GPU and head dim: about 40 MB
+ * at head dim 128.  Calls that share one must not run at the same time: use
+ * one per stream, and one per captured graph if graphs are replayed side by
+ * side.  Creating it synchronises the engine's stream.  After a timeout
+ * (spl_sage_engine_status with SPL_SAGE_DEVERR_TIMEOUT) make a new one. */
 typedef struct spl_sage_kv4_ws spl_sage_kv4_ws;
 int spl_sage_kv4_ws_create(spl_sage* s, spl_sage_kv4_ws** out);
 void spl_sage_kv4_ws_destroy(spl_sage_kv4_ws* ws);
@@ -588,9 +590,13 @@ typedef struct {
  * otherwise all kv_len; window w > 0: only keys after its position - w (and
  * pages wholly before every query's window are not looked at).  A query that
  * sees no key gives zeros and an lse of -infinity.  q is bf16 and already
- * rotated; K and V are the exact cached values; scores, statistics and sums
- * are f32, a probability times its V scale is rounded to bf16 once.  opts: the
- * softmax scale (default 1 / sqrt(head_dim)); NULL = default.  out must not
+ * rotated; K and V are the cached values, scores and lse those of the exact
+ * ones to f32's rounding, sums f32; a probability times its V scale is rounded
+ * to f16 (2^-11).  With max_q * heads / kv_heads above 128 (prompts) each V
+ * value and each probability is, and K scales more than 2^8 apart within 128
+ * keys are rounded by 2^-16 of the largest.  opts: the softmax scale (default
+ * 1 / sqrt(head_dim)) is taken, the smoothing flags are not, a QK LayerNorm is
+ * refused; NULL = default.  The scale must lie in 1e-10 .. 1e10.  out must not
  * overlap q; rows of no sequence are left as they were.  lse: f32
  * [tokens][heads], the natural logarithm of each row's softmax denominator, or
  * NULL.  A bad page id, length or q_start leaves the rows of its sequence
