@@ -108,7 +108,7 @@ int check_cache(const char* call, const spl_sage_kv4* c, int head_dim, sp::Kv4Po
     if ((uintptr_t)c->data % 16) return fail(SPL_SAGE_ERR_INVALID, "%s: the cache must start on 16 bytes", call);
     if (c->kv_heads <= 0 || c->kv_heads > 65535)
         return fail(SPL_SAGE_ERR_INVALID, "%s: %d KV heads", call, c->kv_heads);
-    if (c->pages <= 0 || c->pages * c->page_tokens > 0x7fffffffLL || c->pages > 0x7fffffffLL)
+    if (c->pages <= 0 || c->pages > 0x7fffffffLL || c->pages * c->page_tokens > 0x7fffffffLL)
         return fail(SPL_SAGE_ERR_INVALID, "%s: %lld pages of %d tokens: slots must fit 31 bits", call,
                     (long long)c->pages, c->page_tokens);
     if (c->page_stride % 16 || c->page_stride < block * c->kv_heads)
@@ -330,7 +330,7 @@ int spl_sage_kv4_attend(spl_sage* s, spl_sage_kv4_ws* ws, const spl_sage_kv4* ca
                     (long long)hk);
     if (sh.batch < 0 || sh.batch > MOST) return fail(SPL_SAGE_ERR_INVALID, "%s: %lld sequences", call, (long long)sh.batch);
     if (sh.batch == 0 || sh.tokens == 0) return SPL_SAGE_OK;
-    if (sh.max_q <= 0 || sh.max_q * sh.heads > MOST || sh.max_q > MOST)
+    if (sh.max_q <= 0 || sh.max_q > MOST || sh.max_q * sh.heads > MOST)
         return fail(SPL_SAGE_ERR_INVALID, "%s: at most %lld queries a sequence", call, (long long)sh.max_q);
     if (sh.max_pages <= 0 || sh.max_pages > MOST || sh.max_pages * a.pool.page_tokens > MOST)
         return fail(SPL_SAGE_ERR_INVALID, "%s: %lld pages a sequence", call, (long long)sh.max_pages);

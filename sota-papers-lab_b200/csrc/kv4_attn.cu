@@ -21,7 +21,7 @@
 //     channel sums.  So S is that of the exact cached values, to f32.
 //   - V's n enters the same way.  Its scale goes into the probability, in f16:
 //     p * s * 2^(14 - R), where 2^R bounds the scales the warp has met so far,
-//     is rounded once by 2^-12 of itself (2^-25 * 2^-14 of the largest where it
+//     is rounded once by 2^-11 of itself (2^-25 * 2^-14 of the largest where it
 //     is subnormal); R rises, and the sums are scaled, when a scale comes near
 //     the end of f16's range.  sum(p z) is kept in f32.
 //   - S^T has a key per row, P^T wants the keys along k: movmatrix transposes

@@ -70,7 +70,7 @@ __device__ __forceinline__ int key_hi(const Kv4Attend& a, const Seq& s, int i) {
     return a.causal ? max(0, s.kv - s.qn + i + 1) : s.kv;
 }
 __device__ __forceinline__ int key_lo(const Kv4Attend& a, const Seq& s, int i) {
-    return a.window ? max(0, s.kv - s.qn + i + 1 - a.window) : 0;
+    return a.window ? max(0, max(0, s.kv - s.qn + i + 1) - a.window) : 0;
 }
 
 template <int COLS, int UNIT>
