@@ -42,6 +42,12 @@ constexpr int AT_WARPS = 8, AT_STEP = 32, AT_UNIT = 128;
 // Units a CTA takes at least: all 8 warps get a step (200 cached tokens: 7.0 us
 // instead of 8.6 with 1, 9.8 with 4; 1000: 10.0, 9.2, 11.8).
 constexpr int AT_LEAST = 2;
+// Units that a tile's start and end count for beside its own (two CTAs on an SM
+// and one): 64 sequences of up to 8192 tokens, 32 / 8 heads, D = 128, take 93 us
+// instead of 102 with none (93.8 with 6, 97.6 with 11), 16 of up to 4096, 16 / 16
+// heads, D = 64, 21.8 instead of 28.9; 20 rows in two tiles 40.4 instead of 42
+// (41.2 with 4 and 8).
+constexpr int AT_BEGIN_1 = 4, AT_BEGIN_2 = 6;
 
 template <int D, int NT>
 struct AttnCfg {
@@ -184,7 +190,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
     if (warp == 0) {
         Shares share;
         Piece p;
-        p.any = find_share<COLS, AT_UNIT, AT_LEAST>(a, blockIdx.x, gridDim.x, share, p.at);
+        p.any = find_share<COLS, AT_UNIT, AT_LEAST, NT == 1 ? AT_BEGIN_1 : AT_BEGIN_2>(a, blockIdx.x, gridDim.x, share,
+                                                                                     p.at);
         if (p.any) cut_piece<COLS, AT_UNIT>(a, share, share.first(blockIdx.x), p);
         if (lane == 0) {
             sh = share;
@@ -621,8 +628,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
         __syncthreads();
         if (!whole) {
             // ---- a piece of a split tile: the last to finish joins them
-            const int c0 = p.unit0 ? sh.holder(p.at.start) : blockIdx.x;
-            const int c1 = p.unit1 < p.kr.units ? sh.holder(p.at.start + p.kr.units - 1) : blockIdx.x;
+            const int c0 = first_holder(sh, p), c1 = last_holder(sh, p);
             if (threadIdx.x == 0) sm_last = last_piece(a, c0, c1);
             __syncthreads();
             if (sm_last)

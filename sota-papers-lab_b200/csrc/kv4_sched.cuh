@@ -92,15 +92,20 @@ __device__ __forceinline__ long long seq_units(const Kv4Attend& a, const Seq& s)
     return n;
 }
 
-// U units over `ctas` CTAs, at least `least` to each: the first U mod G of the G
-// that get work have one unit more than the others.
+// All units over `ctas` CTAs, at least `least` to each: the first U mod G of the
+// G that get work have one unit more than the others.  Where every CTA has work
+// a tile counts for `begin` units more, which stand before its own: what its
+// rows, first loads and output cost the CTA that starts it (the kernels say
+// what that brought).
 struct Shares {
     long long U, q, r;  // q = U / G, r = U mod G
     int G;
+    int w;              // units that stand before a tile's own
     Shares() = default;
-    __device__ __forceinline__ Shares(long long units, int ctas, int least) {
-        U = units;
-        G = (int)min(max(U / least, min(U, 1ll)), (long long)ctas);
+    __device__ __forceinline__ Shares(long long units, long long tiles, int ctas, int least, int begin) {
+        G = (int)min(max(units / least, min(units, 1ll)), (long long)ctas);
+        w = units > (long long)least * ctas ? begin : 0;
+        U = units + w * tiles;
         if (U < 1ll << 32) {  // a short division
             q = G ? (uint32_t)U / (uint32_t)G : 0;
         } else {
@@ -120,40 +125,49 @@ struct Shares {
 // Where a unit lies.
 struct Place {
     int b, head, tile;
-    long long start;  // the tile's first unit
+    long long start;  // the tile's first unit, those before its own among them
     Seq s;
 };
 
 // A warp finds CTA `cta`'s share and the tile it begins in (all lanes get it).
 // Lane i holds the lengths of sequence 32 k + i, so up to 32 sequences take one
 // round of loads.  Returns false where the CTA has no work.
-template <int COLS, int UNIT, int LEAST>
+template <int COLS, int UNIT, int LEAST, int BEGIN>
 __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas, Shares& sh, Place& p) {
     const int lane = threadIdx.x & 31, hkv = a.pool.kv_heads;
-    // sequences b0 + lane, their units, and the units up to and with them (one KV head)
+    // sequences b0 + lane, their units, and the units (tiles) up to and with them (one KV head)
     Seq s;
     long long x, incl;
+    int tiles;
     auto scan = [&](int b0) {
         const int b = b0 + lane;
         s = b < a.batch ? seq_at<COLS>(a, b) : Seq{0, 0, 0, 0};
         x = incl = seq_units<COLS, UNIT>(a, s);
+        tiles = s.tiles;
 #pragma unroll
         for (int i = 1; i < 32; i <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, incl, i);
-            if (lane >= i) incl += y;
+            const int t = __shfl_up_sync(0xffffffffu, tiles, i);
+            if (lane >= i) {
+                incl += y;
+                tiles += t;
+            }
         }
     };
-    long long total = 0;
+    long long total = 0, total_tiles = 0;
     for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {  // the first 32 last: they stay
         scan(b0);
         total += __shfl_sync(0xffffffffu, incl, 31);
+        total_tiles += __shfl_sync(0xffffffffu, tiles, 31);
     }
-    sh = Shares(total * hkv, ctas, LEAST);
+    sh = Shares(total * hkv, total_tiles * hkv, ctas, LEAST, BEGIN);
     if (cta >= sh.G) return false;
     const long long u = sh.first(cta);
     long long base = 0;
     for (int b0 = 0;; b0 += 32) {
         if (b0) scan(b0);
+        x += (long long)sh.w * s.tiles;
+        incl += (long long)sh.w * tiles;
         const unsigned over = __ballot_sync(0xffffffffu, base + incl * hkv > u);
         if (over || b0 + 32 >= a.batch) {
             const int w = over ? __ffs(over) - 1 : 0;  // (u < U: there is one)
@@ -172,7 +186,7 @@ __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas
         base += __shfl_sync(0xffffffffu, incl, 31) * hkv;
     }
     for (p.tile = 0; p.tile + 1 < p.s.tiles; p.tile++) {
-        const int n = keys_of<COLS, UNIT>(a, p.s, p.tile).units;
+        const int n = keys_of<COLS, UNIT>(a, p.s, p.tile).units + sh.w;
         if (u < p.start + n) break;
         p.start += n;
     }
@@ -190,17 +204,28 @@ struct Piece {
 template <int COLS, int UNIT>
 __device__ __forceinline__ void cut_piece(const Kv4Attend& a, const Shares& sh, long long from, Piece& p) {
     p.kr = keys_of<COLS, UNIT>(a, p.at.s, p.at.tile);
-    p.unit0 = (int)(from - p.at.start);
-    p.unit1 = (int)min((long long)p.kr.units, sh.first(blockIdx.x + 1) - p.at.start);
+    const long long own = p.at.start + sh.w;
+    p.unit0 = (int)max(0ll, from - own);
+    p.unit1 = (int)min((long long)p.kr.units, sh.first(blockIdx.x + 1) - own);
+    p.any = p.unit0 < p.unit1;  // (not where the share ends before the tile's own units)
+}
+
+// The CTAs that have a piece's tile between them.
+__device__ __forceinline__ int first_holder(const Shares& sh, const Piece& p) {
+    return p.unit0 ? sh.holder(p.at.start + sh.w) : blockIdx.x;
+}
+__device__ __forceinline__ int last_holder(const Shares& sh, const Piece& p) {
+    return p.unit1 < p.kr.units ? sh.holder(p.at.start + sh.w + p.kr.units - 1) : blockIdx.x;
 }
 
 // The piece after p in the CTA's share.
 template <int COLS, int UNIT>
 __device__ __forceinline__ void next_piece(const Kv4Attend& a, const Shares& sh, const Piece& p, Piece& n) {
-    n.any = p.at.start + p.unit1 < sh.first(blockIdx.x + 1);
+    const long long end = p.at.start + sh.w + p.kr.units;
+    n.any = end + sh.w < sh.first(blockIdx.x + 1);
     if (!n.any) return;
     n.at = p.at;
-    n.at.start += p.kr.units;
+    n.at.start = end;
     if (++n.at.tile >= n.at.s.tiles) {
         n.at.tile = 0;
         if (++n.at.head >= a.pool.kv_heads) {
