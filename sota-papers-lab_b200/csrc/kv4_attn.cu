@@ -30,6 +30,13 @@
 // shared memory (cp.async, 16 bytes, no barrier but the warp's own) with its
 // own running maximum and sums; the warps meet once per tile.  Row maxima are
 // looked at by vote and only recomputed when one grows.
+//
+// Measured, 32 / 8 heads, D = 128: one sequence of 131072 tokens (151 MB) 44 us,
+// 64 of up to 8192 (371 MB) 93 us; another 151 MB add 29 us (5.2 TB/s, where a
+// copy reaches 6.45; the issue slots are 3/4 busy).  The rest is a call's start
+// (3 us from the lengths to the first loads), the ends of pieces (about 4 us
+// each, beside the SM's other CTA) and the join (4 us).  One sequence of 1000
+// tokens 9.9 us, all of it such latencies.
 #include <algorithm>
 #include <atomic>
 

@@ -33,7 +33,15 @@
 //
 // The running maximum a row's exponents refer to is only raised when a new one
 // is more than 2^8 larger (P and the sums have room for that), so O is hardly
-// ever rescaled.  Every wait is bounded (sage_dev.cuh): on a timeout all
+// ever rescaled.
+//
+// Measured: 2 x 2048 query tokens on up to 8192 cached ones, 32 / 8 heads, D =
+// 128 (382 GFLOP), 549 us, 695 TFLOP/s, 0.42 of a large bf16 product's rate.
+// No unit bounds it: without the exponentials it took 519 of then 562 us,
+// without the products 520, without the unpacking arithmetic 549; the chain
+// from S to the P that waits for it does.
+//
+// Every wait is bounded (sage_dev.cuh): on a timeout all
 // roles leave their loops, the MMAs in flight are waited for, TMEM is freed.
 #include <atomic>
 
