@@ -906,6 +906,42 @@ def test_attend_prompt_over_a_long_cache_and_shared_pages(engines):
     eng.engine_status()
 
 
+@pytest.mark.parametrize("reserved", [1, 100, 10000])
+def test_attend_with_reserved_sms(engines, reserved):
+    """Fewer CTAs than SMs, down to one SM's, in a workspace that other calls use as well."""
+    d = 128
+    eng = sage.SageAttention(torch.cuda.current_stream(), d)
+    ws = engines["ws", d]
+    if reserved == 10000:
+        reserved = torch.cuda.get_device_properties(0).multi_processor_count - 1
+    eng.reserve_sms(reserved)
+    few = Batch(d, 32, 8, 2, [900, 0, 3, 130], [1, 0, 1, 1], seed=40)
+    some = Batch(d, 32, 8, 2, [500, 260], [4, 5], seed=41)
+    many = Batch(d, 32, 8, 2, [300, 700], [150, 90], seed=42)
+    for b in (few, some, many):
+        b.fill(eng)
+    for _ in range(2):
+        for b in (few, some, many):
+            b.attend(eng, ws)
+            b.attend(engines[d], ws)
+            b.attend(eng, ws)
+    for b in (few, some, many):
+        b.check()
+    eng.engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("hq,hkv,rows", [(160, 1, 1), (129, 1, 1), (128, 1, 1), (16, 2, 16), (16, 2, 17), (6, 2, 3),
+                                         (5, 5, 257)])
+def test_attend_around_the_kernels_limits(engines, d, hq, hkv, rows):
+    """Groups of more heads than a tile has rows, and the row counts where one kernel hands over to the next."""
+    b = Batch(d, 64, hq, hkv, [400, rows, 1], [rows, rows, 1], seed=hq + rows)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], window=99)
+    b.check(window=99)
+    engines[d].engine_status()
+
+
 def test_gpu_refusals(engines):
     """What the wrappers refuse: types, shapes, devices, mixed-up arguments."""
     d, eng, ws = 128, engines[128], engines["ws", 128]
