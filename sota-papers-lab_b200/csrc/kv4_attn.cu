@@ -36,9 +36,10 @@
 // copy reaches 6.45; the issue slots are 3/4 busy).  The rest is a call's start
 // (3 us from the lengths to the first loads), the ends of pieces (about 4 us
 // each, beside the SM's other CTA) and the join (4 us).  One sequence of 1000
-// tokens 9.9 us, all of it such latencies.
+// tokens 8.9 us, all of it such latencies.
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 
 #include "kv4_sched.cuh"
 #include "sage_kernels.h"
@@ -46,8 +47,8 @@
 namespace sp {
 
 constexpr int AT_WARPS = 8, AT_STEP = 32, AT_UNIT = 128;
-// Units a CTA takes at least: all 8 warps get a step (200 cached tokens: 7.0 us
-// instead of 8.6 with 1, 9.8 with 4; 1000: 10.0, 9.2, 11.8).
+// Units a CTA takes at least: all 8 warps get a step (on a full grid, 200 cached
+// tokens: 7.0 us instead of 8.6 with 1, 9.8 with 4; 1000: 10.0, 9.2, 11.8).
 constexpr int AT_LEAST = 2;
 // Units that a tile's start and end count for beside its own (two CTAs on an SM
 // and one): 64 sequences of up to 8192 tokens, 32 / 8 heads, D = 128, take 93 us
@@ -653,7 +654,14 @@ template <int D, int NT>
 static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
     using C = AttnCfg<D, NT>;
     constexpr int COLS = C::COLS;
-    const int G = (NT == 1 ? 2 : 1) * sms;
+    // No more CTAs than the longest sequences that max_pages admits can give
+    // work: those that have some get an SM to themselves then (one sequence of
+    // 200, 1000, 3000 tokens: 6.3, 8.9, 9.3 us instead of 7.1, 10.0, 10.4).
+    // The shares are the same.
+    const int full = (NT == 1 ? 2 : 1) * sms;
+    const double tiles = (double)((a.max_q * a.group + COLS - 1) / COLS) * (a.heads / a.group) * a.batch;
+    const long long units = (((long long)a.max_pages << a.pool.page_shift) + 31 + AT_UNIT - 1) / AT_UNIT;
+    const int G = (int)std::min<double>(full, std::ceil(tiles * units / AT_LEAST));
     if (G * sizeof(uint32_t) > KV4_COUNTS) return cudaErrorInvalidConfiguration;
     a.done = (uint32_t*)a.scratch;
     a.part_ml = (float2*)((uint8_t*)a.scratch + KV4_COUNTS);
