@@ -39,7 +39,6 @@
 // tokens 8.9 us, all of it such latencies.
 #include <algorithm>
 #include <atomic>
-#include <cmath>
 
 #include "kv4_sched.cuh"
 #include "sage_kernels.h"
@@ -47,8 +46,10 @@
 namespace sp {
 
 constexpr int AT_WARPS = 8, AT_STEP = 32, AT_UNIT = 128;
-// Units a CTA takes at least: all 8 warps get a step (on a full grid, 200 cached
-// tokens: 7.0 us instead of 8.6 with 1, 9.8 with 4; 1000: 10.0, 9.2, 11.8).
+// Units a CTA takes at least: all 8 warps get a step (one sequence of 200 tokens
+// 6.2 us, with one unit 8.2, of 1000 8.9 and 8.6, of 3000 9.2 and 10.8).  Where no
+// CTA gets more, none gets parts of two tiles (6000 tokens: 11.6 us instead of
+// 16.8, 9000: 12.6 and 18.8).
 constexpr int AT_LEAST = 2;
 // Units that a tile's start and end count for beside its own (two CTAs on an SM
 // and one): 64 sequences of up to 8192 tokens, 32 / 8 heads, D = 128, take 93 us
@@ -661,7 +662,7 @@ static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
     const int full = (NT == 1 ? 2 : 1) * sms;
     const double tiles = (double)((a.max_q * a.group + COLS - 1) / COLS) * (a.heads / a.group) * a.batch;
     const long long units = (((long long)a.max_pages << a.pool.page_shift) + 31 + AT_UNIT - 1) / AT_UNIT;
-    const int G = (int)std::min<double>(full, std::ceil(tiles * units / AT_LEAST));
+    const int G = (int)std::min<double>(full, tiles * ((units + AT_LEAST - 1) / AT_LEAST));
     if (G * sizeof(uint32_t) > KV4_COUNTS) return cudaErrorInvalidConfiguration;
     a.done = (uint32_t*)a.scratch;
     a.part_ml = (float2*)((uint8_t*)a.scratch + KV4_COUNTS);

@@ -85,27 +85,38 @@ __device__ __forceinline__ KeyRange keys_of(const Kv4Attend& a, const Seq& s, in
     return r;
 }
 
-template <int COLS, int UNIT>
-__device__ __forceinline__ long long seq_units(const Kv4Attend& a, const Seq& s) {
+// A sequence's units (one KV head); `more`: its tiles, and in the upper half
+// the units missing to multiples of LEAST per tile.
+template <int COLS, int UNIT, int LEAST>
+__device__ __forceinline__ long long seq_units(const Kv4Attend& a, const Seq& s, uint64_t& more) {
+    static_assert((LEAST & (LEAST - 1)) == 0, "a power of two");
     long long n = 0;
-    for (int t = 0; t < s.tiles; t++) n += keys_of<COLS, UNIT>(a, s, t).units;
+    more = 0;
+    for (int t = 0; t < s.tiles; t++) {
+        const int units = keys_of<COLS, UNIT>(a, s, t).units;
+        n += units;
+        more += 1 + ((uint64_t)(-units & (LEAST - 1)) << 32);
+    }
     return n;
 }
 
-// All units over `ctas` CTAs, at least `least` to each: the first U mod G of the
-// G that get work have one unit more than the others.  Where every CTA has work
-// a tile counts for `begin` units more, which stand before its own: what its
-// rows, first loads and output cost the CTA that starts it (the kernels say
-// what that brought).
+// All units over `ctas` CTAs.  Where they do not give every CTA `least`, each
+// tile is made a multiple of that many, so that no CTA works on two tiles one
+// after the other.  Where they do, the first U mod G CTAs have one unit more than
+// the others, and a tile counts for `begin` units more, which stand before its
+// own: what its rows, first loads and output cost the CTA that starts it (the
+// kernels say what either brought).
 struct Shares {
     long long U, q, r;  // q = U / G, r = U mod G
-    int G;
-    int w;              // units that stand before a tile's own
+    int G;              // CTAs that get work
+    int w, pad;         // units that stand before a tile's own; its own are rounded up to a multiple of pad + 1
     Shares() = default;
-    __device__ __forceinline__ Shares(long long units, long long tiles, int ctas, int least, int begin) {
-        G = (int)min(max(units / least, min(units, 1ll)), (long long)ctas);
-        w = units > (long long)least * ctas ? begin : 0;
-        U = units + w * tiles;
+    __device__ __forceinline__ Shares(long long units, long long missing, long long tiles, int ctas, int least, int begin) {
+        const bool few = units + missing <= (long long)least * ctas;
+        w = few ? 0 : begin;
+        pad = few ? least - 1 : 0;
+        U = few ? units + missing : units + w * tiles;
+        G = few ? (int)(U / least) : ctas;
         if (U < 1ll << 32) {  // a short division
             q = G ? (uint32_t)U / (uint32_t)G : 0;
         } else {
@@ -120,6 +131,7 @@ struct Shares {
         const int base = u < wide ? 0 : (int)r;
         return base + (x < 1ll << 32 ? (int)((uint32_t)x / (uint32_t)per) : (int)(x / per));
     }
+    __device__ __forceinline__ int of_tile(int units) const { return w + ((units + pad) & ~pad); }
 };
 
 // Where a unit lies.
@@ -135,39 +147,41 @@ struct Place {
 template <int COLS, int UNIT, int LEAST, int BEGIN>
 __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas, Shares& sh, Place& p) {
     const int lane = threadIdx.x & 31, hkv = a.pool.kv_heads;
-    // sequences b0 + lane, their units, and the units (tiles) up to and with them (one KV head)
+    // sequences b0 + lane, their units, and those up to and with them (one KV head)
     Seq s;
     long long x, incl;
-    int tiles;
+    uint64_t more, more_incl;
     auto scan = [&](int b0) {
         const int b = b0 + lane;
         s = b < a.batch ? seq_at<COLS>(a, b) : Seq{0, 0, 0, 0};
-        x = incl = seq_units<COLS, UNIT>(a, s);
-        tiles = s.tiles;
+        x = incl = seq_units<COLS, UNIT, LEAST>(a, s, more);
+        more_incl = more;
 #pragma unroll
         for (int i = 1; i < 32; i <<= 1) {
             const long long y = __shfl_up_sync(0xffffffffu, incl, i);
-            const int t = __shfl_up_sync(0xffffffffu, tiles, i);
+            const uint64_t z = __shfl_up_sync(0xffffffffu, more_incl, i);
             if (lane >= i) {
                 incl += y;
-                tiles += t;
+                more_incl += z;
             }
         }
     };
-    long long total = 0, total_tiles = 0;
+    long long total = 0, missing = 0, tiles = 0;
     for (int b0 = (a.batch - 1) & ~31; b0 >= 0; b0 -= 32) {  // the first 32 last: they stay
         scan(b0);
         total += __shfl_sync(0xffffffffu, incl, 31);
-        total_tiles += __shfl_sync(0xffffffffu, tiles, 31);
+        const uint64_t m = __shfl_sync(0xffffffffu, more_incl, 31);
+        tiles += (uint32_t)m;
+        missing += m >> 32;
     }
-    sh = Shares(total * hkv, total_tiles * hkv, ctas, LEAST, BEGIN);
+    sh = Shares(total * hkv, missing * hkv, tiles * hkv, ctas, LEAST, BEGIN);
     if (cta >= sh.G) return false;
     const long long u = sh.first(cta);
     long long base = 0;
     for (int b0 = 0;; b0 += 32) {
         if (b0) scan(b0);
-        x += (long long)sh.w * s.tiles;
-        incl += (long long)sh.w * tiles;
+        x += sh.pad ? (long long)(more >> 32) : (long long)sh.w * (uint32_t)more;
+        incl += sh.pad ? (long long)(more_incl >> 32) : (long long)sh.w * (uint32_t)more_incl;
         const unsigned over = __ballot_sync(0xffffffffu, base + incl * hkv > u);
         if (over || b0 + 32 >= a.batch) {
             const int w = over ? __ffs(over) - 1 : 0;  // (u < U: there is one)
@@ -186,7 +200,7 @@ __device__ __forceinline__ bool find_share(const Kv4Attend& a, int cta, int ctas
         base += __shfl_sync(0xffffffffu, incl, 31) * hkv;
     }
     for (p.tile = 0; p.tile + 1 < p.s.tiles; p.tile++) {
-        const int n = keys_of<COLS, UNIT>(a, p.s, p.tile).units + sh.w;
+        const int n = sh.of_tile(keys_of<COLS, UNIT>(a, p.s, p.tile).units);
         if (u < p.start + n) break;
         p.start += n;
     }
@@ -221,7 +235,7 @@ __device__ __forceinline__ int last_holder(const Shares& sh, const Piece& p) {
 // The piece after p in the CTA's share.
 template <int COLS, int UNIT>
 __device__ __forceinline__ void next_piece(const Kv4Attend& a, const Shares& sh, const Piece& p, Piece& n) {
-    const long long end = p.at.start + sh.w + p.kr.units;
+    const long long end = p.at.start + sh.of_tile(p.kr.units);
     n.any = end + sh.w < sh.first(blockIdx.x + 1);
     if (!n.any) return;
     n.at = p.at;
