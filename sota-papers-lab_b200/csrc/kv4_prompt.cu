@@ -168,11 +168,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
     // Pieces, made one ahead by the unpacking warps, which are at most two
     // key tiles (so two pieces) ahead of the softmax.
     __shared__ Piece pieces[RING];
-    __shared__ float sm_amax[PR_SOFTMAX];
+    __shared__ int8_t sm_up[PR_ROWS];  // the power of two that each row of Q was scaled by
     // The largest scales and zeros of a tile, as bf16 bits (zero in the upper half), of each unpacking warp's part
     __shared__ uint2 sm_top[2][PR_UNPACK];
-    __shared__ float sm_f[4];  // of a tile: what its S is multiplied by
-    __shared__ int sm_R[4];    // ... and the R of its V
+    __shared__ int sm_E[4];  // of a tile: its K was scaled by 2^-E
+    __shared__ int sm_R[4];  // ... and its V by 2^-R
     __shared__ float2 sm_join[PR_SOFTMAX * 32 / (D / 4)];
     __shared__ bool sm_last;
     __shared__ volatile uint32_t sm_gave_up;  // a wait of this CTA ran out
@@ -249,17 +249,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             const int n = p.unit1 - p.unit0, n0 = p.at.tile * PR_ROWS, rows = s.qn * a.group;
             const bool two = n0 + 128 < rows;  // B has rows
             const int nr = n0 + x * 128 + row;
-            // ---- the rows of Q, scaled by the power of two that brings the
-            // piece's largest finite magnitude to [2^13, 2^14) (bf16 values
-            // down to 2^-28 of it stay exact; what is not finite stays in its
-            // own row), channels of each 8 in the order 0 4 1 5 2 6 3 7 (that
-            // of K's nibbles)
+            // ---- the rows of Q, each scaled by the power of two that brings
+            // its largest magnitude to [2^13, 2^14) (bf16 values down to 2^-28
+            // of it stay exact), channels of each 8 in the order 0 4 1 5 2 6
+            // 3 7 (that of K's nibbles)
             {
                 // D/8 lanes hold a row's 16-byte pieces: 256/D rows of the warp's 32 at a time
                 constexpr int PIECES = D / 8, AT_ONCE = 32 / PIECES, TURNS = 32 / AT_ONCE;
                 const int piece = lane % PIECES, gr = piece / 8;
                 uint4 w[TURNS];
-                float amax = 0.f;
 #pragma unroll
                 for (int i = 0; i < TURNS; i++) {
                     const int m = nr - lane + i * AT_ONCE + lane / PIECES, tok = by_group(a, min(m, rows - 1));
@@ -269,42 +267,46 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                                                 (p.at.head * a.group + m - tok * a.group) * a.q.sh) + piece);
                 }
 #pragma unroll
-                for (int i = 0; i < TURNS; i++) {
-                    float f[8];
-                    unpack_bf16x8(w[i], f);
+                for (int i = 0; i < TURNS; i += 2) {
+                    // the largest magnitudes of two turns' rows, as bf16 bits
+                    uint32_t top[2];
 #pragma unroll
-                    for (int j = 0; j < 8; j++) amax = fmaxf(amax, fabsf(f[j]) < INFINITY ? fabsf(f[j]) : 0.f);
-                }
-                amax = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(amax)));
-                if (lane == 0) sm_amax[warp] = amax;
-                named_bar(1, PR_SOFTMAX * 32);
-#pragma unroll
-                for (int i = 0; i < PR_SOFTMAX; i++) amax = fmaxf(amax, sm_amax[i]);
-                const float up = exp2i(min(max(13 - expo(amax), -100), 100));
-#pragma unroll
-                for (int i = 0; i < TURNS; i++) {
-                    const int m = (warp & 3) * 32 + i * AT_ONCE + lane / PIECES;
-                    float f[8], sum = 0.f;
-                    unpack_bf16x8(w[i], f);
-#pragma unroll
-                    for (int j = 0; j < 8; j++) {
-                        f[j] *= up;
-                        sum += f[j];
+                    for (int j = 0; j < 2; j++) {
+                        const uint4 v = w[i + j];
+                        top[j] = umax2(umax2(v.x & 0x7fff7fffu, v.y & 0x7fff7fffu), umax2(v.z & 0x7fff7fffu, v.w & 0x7fff7fffu));
                     }
-                    sts128(base + C::Q_OFF + x * C::Q + gr * C::ATOM + m * 128 + (((piece & 7) ^ (m & 7)) << 4),
-                           half2_bits(f[0], f[4]), half2_bits(f[1], f[5]), half2_bits(f[2], f[6]), half2_bits(f[3], f[7]));
-                    // the sum over the group, (hi, lo, hi, lo)
+                    uint32_t both = umax2(__byte_perm(top[0], top[1], 0x5410), __byte_perm(top[0], top[1], 0x7632));
 #pragma unroll
-                    for (int j = 1; j < 8; j <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, j);
-                    const uint32_t both = split_half(sum * 0x1p-8f);
-                    uint8_t* qx = sm + C::QX_OFF + x * C::X + m * 32 + ((m >> 2 & 1) << 4);
-                    if ((piece & 7) == 0) *(uint2*)(qx + gr * 8) = make_uint2(both, both);
-                    if (NG == 1 && piece == 1) *(uint2*)(qx + 8) = make_uint2(0, 0);
+                    for (int j = 1; j < PIECES; j <<= 1) both = umax2(both, __shfl_xor_sync(0xffffffffu, both, j));
+#pragma unroll
+                    for (int j = 0; j < 2; j++) {
+                        const int m = (warp & 3) * 32 + (i + j) * AT_ONCE + lane / PIECES;
+                        const int k = min(max(13 - bexpo(both >> 16 * j), -100), 100);
+                        const float up = exp2i(k);
+                        float f[8], sum = 0.f;
+                        unpack_bf16x8(w[i + j], f);
+#pragma unroll
+                        for (int n = 0; n < 8; n++) {
+                            f[n] *= up;
+                            sum += f[n];
+                        }
+                        sts128(base + C::Q_OFF + x * C::Q + gr * C::ATOM + m * 128 + (((piece & 7) ^ (m & 7)) << 4),
+                               half2_bits(f[0], f[4]), half2_bits(f[1], f[5]), half2_bits(f[2], f[6]), half2_bits(f[3], f[7]));
+                        // the sum over the group, (hi, lo, hi, lo)
+#pragma unroll
+                        for (int n = 1; n < 8; n <<= 1) sum += __shfl_xor_sync(0xffffffffu, sum, n);
+                        const uint32_t twice = split_half(sum * 0x1p-8f);
+                        uint8_t* qx = sm + C::QX_OFF + x * C::X + m * 32 + ((m >> 2 & 1) << 4);
+                        if ((piece & 7) == 0) *(uint2*)(qx + gr * 8) = make_uint2(twice, twice);
+                        if (NG == 1 && piece == 1) *(uint2*)(qx + 8) = make_uint2(0, 0);
+                        if (piece == 0) sm_up[x * 128 + m] = (int8_t)k;
+                    }
                 }
                 fence_proxy_async_smem();
                 __syncwarp();
                 if (lane == 0) mbar_arrive(bar(bars.q_full));
             }
+            const int up_row = sm_up[x * 128 + row];  // (of the warp's own rows)
             if (x == 0 || two) {
                 float m_ref = -INFINITY, l = 0.f;  // the row's (log2) reference and sum
                 int R_ref = 0;                     // O holds sum(p v) * 2^(7 - R_ref)
@@ -353,7 +355,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         const bool edge = key0 + PR_KEYS > all_hi || key0 < all_lo;
                         const int R = sm_R[tj & 3];
                         bool raise = j == 0 || R > R_ref;  // (the same in all rows)
-                        const float f = sm_f[tj & 3];
+                        // what S is multiplied by: softmax scale times 2^(E - up), in two steps (either may be far from 1)
+                        const int e = sm_E[tj & 3] - up_row;
+                        const float f = fminf(fmaxf(a.c * exp2i(e >> 1) * exp2i(e - (e >> 1)), 1e-37f), 3e38f);
 #pragma unroll 1
                         for (int h = 0; h < 2; h++) {
                             uint32_t r[2][32];
@@ -622,7 +626,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             load_params();
             kid = k_id(2);
             vid = v_id(2);
-            float factor = 0.f;  // softmax scale, without the power of two that Q was scaled by
             for (int j = 0; j < n; j++) {
                 const uint32_t tj = t + j, st = tj & 1;
                 // ---- the tile's powers of two, from the bf16 bits of all scales and zeros
@@ -686,16 +689,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                                hfma2(hi & 0x000f000fu, sl, off), hfma2(hi & 0x00f000f0u, sh_, off));
                     }
                 }
-                if (j == 0) {
-                    if (w == 0) sm_go[2][events & 1] = warp_all_wait(bar(bars.q_full), turn & 1, a.err, 64) && !sm_gave_up;
-                    named_bar(2, PR_UNPACK * 32);
-                    ok = sm_go[2][events++ & 1];
-                    if (!ok) break;
-                    float amax = 0.f;
-#pragma unroll
-                    for (int i = 0; i < PR_SOFTMAX; i++) amax = fmaxf(amax, sm_amax[i]);
-                    factor = a.c * exp2i(-min(max(13 - expo(amax), -100), 100));
-                }
                 if (kh == 0) {
                     // (hi, hi, lo, lo) of each group, against the row's (hi, lo, hi, lo)
                     uint32_t cw[2] = {0, 0};
@@ -706,7 +699,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     sts128(base + C::KX_OFF + st * C::X + kk * 32 + ((kk >> 2 & 1) << 4), __byte_perm(cw[0], 0, 0x1010),
                            __byte_perm(cw[0], 0, 0x3232), __byte_perm(cw[1], 0, 0x1010), __byte_perm(cw[1], 0, 0x3232));
                     if (w == 0 && lane == 0) {
-                        sm_f[tj & 3] = fmaxf(factor * exp2i(E), 1e-37f);
+                        sm_E[tj & 3] = E;
                         sm_R[tj & 3] = R;
                     }
                 }

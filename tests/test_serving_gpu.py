@@ -988,3 +988,25 @@ def test_gpu_refusals(engines):
     with pytest.raises(sage.SageError):
         eng.kv4_attend(closed, cache, q, o, ids, kv)
     eng.engine_status()
+
+
+# ---------------------------------------------------------------- magnitudes, signs, joins
+
+def large_query(engines, d, size, rows):
+    """One query row far larger than the others, which do not change by a bit."""
+    b = Batch(d, 16, 4, 2, [300], [rows], seed=rows, tail_rows=0)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    right = b.out.clone()
+    b.q[rows // 2, 1] *= size
+    b.attend(engines[d], engines["ws", d])
+    hit = torch.zeros(rows, 4, dtype=torch.bool, device=DEV)
+    hit[rows // 2, 1] = True
+    assert torch.equal(b.out[~hit], right[~hit]) and torch.isfinite(b.out).all()
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [3, 5, 90])
+def test_attend_large_queries_leave_other_rows_alone(engines, d, rows):
+    large_query(engines, d, 1e4, rows)
