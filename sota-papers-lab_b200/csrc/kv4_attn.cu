@@ -115,6 +115,11 @@ __device__ __forceinline__ uint2 lds64(uint32_t p) {
     asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(p));
     return v;
 }
+__device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
+    uint64_t d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
+    return d;
+}
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
@@ -492,11 +497,14 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
                         }
                     }
             }
-            float mc[NT][2];
+            // Probabilities are 2^((x - m) cf), the difference first: x cf - (m cf) as one fused step would leave the
+            // rounding of m cf in the exponent, which outgrows f32's range where scores pass 2^30.
+            uint64_t less[NT], by[NT];
 #pragma unroll
-            for (int nt = 0; nt < NT; nt++)
-#pragma unroll
-                for (int j = 0; j < 2; j++) mc[nt][j] = m[nt][j] == -INFINITY ? 0.f : m[nt][j] * cf[nt][j];
+            for (int nt = 0; nt < NT; nt++) {
+                less[nt] = pk2(m[nt][0] == -INFINITY ? 0.f : -m[nt][0], m[nt][1] == -INFINITY ? 0.f : -m[nt][1]);
+                by[nt] = pk2(cf[nt][0], cf[nt][1]);
+            }
 
             // ---- V's scales within f16's reach
             float top[NG];
@@ -532,13 +540,17 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                 for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
-                    for (int i4 = 0; i4 < 4; i4++) {
-                        const int r = i4 >> 1, j = i4 & 1;
-                        const float p = ex2(fmaf(x[h][nt][i4], cf[nt][j], -mc[nt][j]));
-                        x[h][nt][i4] = p;
-                        l[nt][j] += p;
+                    for (int r = 0; r < 2; r++) {
+                        float y[2];
+                        upk2(mul2(add2(pk2(x[h][nt][2 * r], x[h][nt][2 * r + 1]), less[nt]), by[nt]), y[0], y[1]);
 #pragma unroll
-                        for (int gr = 0; gr < NG; gr++) zs[nt][gr][j] = fmaf(p, vz[h][r][gr], zs[nt][gr][j]);
+                        for (int j = 0; j < 2; j++) {
+                            const float p = ex2(y[j]);
+                            x[h][nt][2 * r + j] = p;
+                            l[nt][j] += p;
+#pragma unroll
+                            for (int gr = 0; gr < NG; gr++) zs[nt][gr][j] = fmaf(p, vz[h][r][gr], zs[nt][gr][j]);
+                        }
                     }
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++)

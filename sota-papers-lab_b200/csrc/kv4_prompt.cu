@@ -118,7 +118,6 @@ __device__ __forceinline__ void tmem_st16(uint32_t taddr, const uint32_t (&r)[16
         : "memory");
 }
 __device__ __forceinline__ float exp2i(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }  // -126 .. 127
-__device__ __forceinline__ int expo(float x) { return (int)(__float_as_uint(x) >> 23 & 255) - 127; }
 __device__ __forceinline__ uint32_t half2_bits(float lo, float hi) {
     uint32_t r;
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
@@ -308,7 +307,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             }
             const int up_row = sm_up[x * 128 + row];  // (of the warp's own rows)
             if (x == 0 || two) {
-                float m_ref = -INFINITY, l = 0.f;  // the row's (log2) reference and sum
+                float m_ref = -INFINITY, l = 0.f;  // the row's reference, as q k, and sum
                 int R_ref = 0;                     // O holds sum(p v) * 2^(7 - R_ref)
                 uint32_t poison = 0;               // groups of V that reach the row as NaN
                 const int tok = by_group(a, min(nr, rows - 1));
@@ -358,6 +357,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         // what S is multiplied by: softmax scale times 2^(E - up), in two steps (either may be far from 1)
                         const int e = sm_E[tj & 3] - up_row;
                         const float f = fminf(fmaxf(a.c * exp2i(e >> 1) * exp2i(e - (e >> 1)), 1e-37f), 3e38f);
+                        float m_s = m_ref * exp2i(-e >> 1) * exp2i(-e - (-e >> 1));  // the reference in S's units
 #pragma unroll 1
                         for (int h = 0; h < 2; h++) {
                             uint32_t r[2][32];
@@ -380,12 +380,15 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
 #pragma unroll
                                 for (int i = 0; i < 32; i += 2)
                                     mx[i / 2 & 3] = max3(mx[i / 2 & 3], __uint_as_float(r[ch][i]), __uint_as_float(r[ch][i + 1]));
-                            const float top = f * fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
+                            const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
                             // ---- a new reference, where the maximum has outgrown the last by 2^8; a new R
-                            const bool grew = top > m_ref + 8.f;  // (from -infinity: any)
+                            const bool grew = f * (top - m_s) > 8.f;  // (from -infinity: any)
                             if (__any_sync(0xffffffffu, grew) || raise) {
-                                float fo = grew ? ex2(m_ref - top) : 1.f;
-                                if (grew) m_ref = top;
+                                float fo = grew ? ex2(f * (m_s - top)) : 1.f;
+                                if (grew) {
+                                    m_s = top;
+                                    m_ref = top * exp2i(e >> 1) * exp2i(e - (e >> 1));
+                                }
                                 l *= fo;
                                 if (raise) {
                                     if (j > 0) fo *= exp2i(max(R_ref - (R + 2), -126));
@@ -410,10 +413,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                                     }
                                 }
                             }
-                            // ---- P = 2^(S f - ref + shift), packed over S
+                            // ---- P = 2^((S - ref) f + shift), packed over S.  (The difference first: the rounding of ref f
+                            // in the exponent of a fused S f - ref f outgrows f32 where scores pass 2^30.)
                             const int shift = max(7 + R - R_ref, -100);  // at most 5
-                            const float less = (float)shift - (m_ref == -INFINITY ? 0.f : m_ref);
-                            const uint64_t less2 = pk2(less, less), f2 = pk2(f, f);
+                            const float less = m_s == -INFINITY ? 0.f : -m_s, up = (float)shift;
+                            const uint64_t less2 = pk2(less, less), f2 = pk2(f, f), up2 = pk2(up, up);
                             uint64_t sum2[2] = {0, 0};
 #pragma unroll
                             for (int ch = 0; ch < 2; ch++) {
@@ -421,7 +425,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
 #pragma unroll
                                 for (int i = 0; i < 16; i++) {
                                     float u, v;
-                                    upk2(fma2(pk2(__uint_as_float(r[ch][2 * i]), __uint_as_float(r[ch][2 * i + 1])), f2, less2), u, v);
+                                    upk2(fma2(add2(pk2(__uint_as_float(r[ch][2 * i]), __uint_as_float(r[ch][2 * i + 1])), less2), f2, up2), u, v);
                                     u = ex2(u);
                                     v = ex2(v);
                                     sum2[i & 1] = add2(sum2[i & 1], pk2(u, v));
@@ -506,10 +510,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     }
                     if (nr < rows) {
                         if (!whole)
-                            a.part_ml[part_row] = make_float2(m_ref, l);
+                            a.part_ml[part_row] = make_float2(a.c * m_ref, l);
                         else if (a.lse)
                             a.lse[(long long)(s.row0 + tok) * a.heads + h] =
-                                ((m_ref == -INFINITY ? 0.f : m_ref) + log2f(l)) * 0.6931471805599453f;
+                                ((m_ref == -INFINITY ? 0.f : a.c * m_ref) + log2f(l)) * 0.6931471805599453f;
                     }
                     tc_fence_before();
                 }

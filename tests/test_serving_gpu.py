@@ -1010,3 +1010,83 @@ def large_query(engines, d, size, rows):
 @pytest.mark.parametrize("rows", [3, 5, 90])
 def test_attend_large_queries_leave_other_rows_alone(engines, d, rows):
     large_query(engines, d, 1e4, rows)
+
+
+def exact_attend(b, causal=True, window=0):
+    """Per sequence with queries: its first row, 64-bit outputs [token][head][D], lse, and what a rounding can be
+    relative to: the probabilities' products with the largest magnitude that a stored group can hold."""
+    d, hkv, g = b.d, b.hkv, b.hq // b.hkv
+    kh, vh = held(b.pool, b.page, d)
+    row = 0
+    for i, (n, qn) in enumerate(zip(b.kv, b.qn)):
+        if qn and n:
+            p = b.pages[i, :-(-n // b.page)].long()
+            k, v = (x[p].transpose(1, 2).reshape(-1, hkv, d)[:n] for x in (kh, vh))
+            top = v.unflatten(-1, (-1, 64)).abs().amax(-1).repeat_interleave(64, -1)
+            j, at = torch.arange(n, device=DEV), n - qn + torch.arange(qn, device=DEV)[:, None]
+            see = torch.ones(qn, n, dtype=torch.bool, device=DEV)
+            if causal:
+                see &= j <= at
+            if window:
+                see &= j > at - window
+            q = b.q[row:row + qn].double().unflatten(1, (hkv, g))
+            x = torch.einsum("thgd,khd->thgk", q, k) * d ** -0.5
+            x = torch.where(see[:, None, None], x, -math.inf)
+            lse = torch.logsumexp(x, -1)
+            most = x.amax(-1, keepdim=True)
+            pr = torch.exp(x - torch.where(most == -math.inf, 0.0, most))
+            pr = pr / pr.sum(-1, keepdim=True).clamp(min=1e-300)
+            o, size = (torch.einsum("thgk,khd->thgd", pr, y).flatten(1, 2) for y in (v, top))
+            yield row, o, lse.flatten(1, 2), size
+        row += qn
+
+
+def check_attend(b, what, **k):
+    """Against 64 bits: the output's rounding to bf16 (2^-8 of it), and of probabilities and values on the way (each
+    key's part by 2^-9 of the most that its group of channels can be), scores' f32 sums (2^-15 of what they weigh:
+    |scores| here are below 2^7 where they count, 2^-24 each way of up to 2^2 terms)."""
+    for row, o, lse, size in exact_attend(b, **k):
+        got = b.out[row:row + o.shape[0]].double()
+        assert torch.isfinite(got).all(), (what, (~torch.isfinite(got)).nonzero()[:4].tolist())
+        bad = (got - o).abs() > 2.0 ** -8 * o.abs() + (2.0 ** -9 + 2.0 ** -15) * size + 1e-30
+        assert not bad.any(), (what, bad.nonzero()[:4].tolist(), float((got - o).abs().max()))
+        gl = b.lse[row:row + o.shape[0]].double()
+        assert ((gl == lse) | ((gl - lse).abs() <= 2.0 ** -15 + 2.0 ** -20 * lse.abs())).all(), (what, "lse")
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e12, 1e30])
+@pytest.mark.parametrize("rows", [1, 5, 90])
+def test_attend_scores_far_beyond_one(engines, d, size, rows):
+    """Scores of up to 1e31: each row is the value of its best key, as far ahead of the second as they are large; of two
+    equal keys, the mean."""
+    b = Batch(d, 16, 4, 2, [400], [rows], seed=rows + d, tail_rows=0)
+    b.k = (b.k.float() * size).bfloat16()
+    for h in range(4):  # (a best key that is clearly the best)
+        b.k[7 + 90 * h, h // 2] = (b.q[:rows, h].float().mean(0) * 8 * size).bfloat16()
+    b.k[350] = b.k[7]
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    assert torch.isfinite(b.out).all()
+    for row, o, lse, size64 in exact_attend(b):
+        kh, _ = held(b.pool, b.page, d)
+        p = b.pages[0, :25].long()
+        k = kh[p].transpose(1, 2).reshape(-1, 2, d)[:400]
+        x = torch.einsum("thgd,khd->thgk", b.q.double().unflatten(1, (2, 2)), k).flatten(1, 2)
+        two = x.topk(3, -1).values
+        # rows whose third score is behind by more than f32's rounding of scores can make up
+        clear = (two[..., 0] - two[..., 2]) * d ** -0.5 > 40 + 2.0 ** -16 * two.abs().amax(-1) * d ** -0.5
+        same = (two[..., 0] == two[..., 1]) | ((two[..., 0] - two[..., 1]) * d ** -0.5 > 40 + 2.0 ** -16 * two.abs().amax(-1))
+        fine = clear & same & (x.abs().amax(-1) == two[..., 0].abs())
+        got = b.out[row:row + rows].double()
+        bad = ((got - o).abs() > 2.0 ** -8 * o.abs() + 2.0 ** -9 * size64) & fine[..., None]
+        assert not bad.any()
+        assert ((b.lse[row:row + rows].double() - lse).abs() <= 2.0 ** -18 * lse.abs() + 1e-4).all()
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e12, 1e30])
+@pytest.mark.parametrize("rows", [3, 5, 90])
+def test_attend_huge_queries_leave_other_rows_alone(engines, d, size, rows):
+    large_query(engines, d, size, rows)
