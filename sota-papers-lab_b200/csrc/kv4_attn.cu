@@ -511,7 +511,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
             bool over = false;
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
-                top[gr] = fmaxf(fmaxf(vs[0][0][gr], vs[0][1][gr]), fmaxf(vs[1][0][gr], vs[1][1][gr]));
+                top[gr] = fmaxf(fmaxf(fabsf(vs[0][0][gr]), fabsf(vs[0][1][gr])), fmaxf(fabsf(vs[1][0][gr]), fabsf(vs[1][1][gr])));
                 over = over || top[gr] > v_lim[gr];
             }
             if (__any_sync(0xffffffffu, over)) {

@@ -1090,3 +1090,21 @@ def test_attend_scores_far_beyond_one(engines, d, size, rows):
 @pytest.mark.parametrize("rows", [3, 5, 90])
 def test_attend_huge_queries_leave_other_rows_alone(engines, d, size, rows):
     large_query(engines, d, size, rows)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 6, 70])
+def test_attend_scales_of_either_sign(engines, d, rows):
+    """A pool that another program wrote: half of the scales negative (the largest of them the largest of all)."""
+    b = Batch(d, 16, 8, 2, [500], [rows], seed=rows, tail_rows=0)
+    b.v[::3] *= 8
+    b.fill(engines[d])
+    _, _, kp, vp = parts(b.pool.cpu().numpy(), b.page, d)
+    half, par = b.page * d // 2, b.page * d // 64 * 4
+    for i, p in enumerate((kp, vp)):
+        p[..., 0::2, :, 0] ^= 0x8000  # every second token's scales
+        at = 2 * half + i * par
+        b.pool[..., at:at + par] = torch.from_numpy(p.reshape(*p.shape[:2], -1).view(np.uint8)).to(DEV)
+    b.attend(engines[d], engines["ws", d])
+    check_attend(b, "signs")
+    engines[d].engine_status()
