@@ -20,10 +20,12 @@
 //     sum is kept apart and S = s0 a0 + s1 a1 + (z0 Q0 + z1 Q1), Q the row's
 //     channel sums.  So S is that of the exact cached values, to f32.
 //   - V's n enters the same way.  Its scale goes into the probability, in f16:
-//     p * s * 2^(14 - R), where 2^R bounds the scales the warp has met so far,
-//     is rounded once by 2^-11 of itself (2^-25 * 2^-14 of the largest where it
-//     is subnormal); R rises, and the sums are scaled, when a scale comes near
-//     the end of f16's range.  sum(p z) is kept in f32.
+//     p * s * 2^(14 - R) is rounded once by 2^-11 of itself (2^-25 * 2^-14 of
+//     2^R where it is subnormal).  R follows the magnitudes of the scales that
+//     the warp meets, within [2^(R - 16), 2^(R + 1)]; the few keys of a step
+//     whose scale lies outside while others' do not are added to the sums in
+//     f32, one by one, so that no key takes precision from the rows that do
+//     not see it.  sum(p z) is kept in f32.
 //   - S^T has a key per row, P^T wants the keys along k: movmatrix transposes
 //     the 8x8 blocks in registers.
 // Each of the 8 warps streams its own 32-key steps through its own ring in
@@ -120,6 +122,17 @@ __device__ __forceinline__ uint64_t mul2(uint64_t a, uint64_t b) {
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d) : "l"(a), "l"(b));
     return d;
 }
+// Halves of 16 bits: maxima, sums without a carry between them.
+__device__ __forceinline__ uint32_t umax2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+__device__ __forceinline__ uint32_t uadd2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
 __device__ __forceinline__ float bf_lo(uint32_t w) { return __uint_as_float(w << 16); }
 __device__ __forceinline__ float bf_hi(uint32_t w) { return __uint_as_float(w & 0xffff0000u); }
 
@@ -169,6 +182,95 @@ __device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, co
     }
 }
 
+// V's scales in f16: R with 2^(R - 16) <= |s| < 2^(R + 1) for those that are held (as bf16 bits less `low`, at
+// most V_SPAN; bits of another sign or of NaN are not).
+constexpr uint32_t V_SPAN = (17u << 7) * 0x10001u, V_UNSET = 0x80008000u;
+// |s|, 0 where it is not finite (such a key comes out as NaN in the rows that see it whatever R is).
+__device__ __forceinline__ float scale_size(float s) { return fabsf(s) < INFINITY ? fabsf(s) : 0.f; }
+__device__ __forceinline__ int scale_R(float top) { return max((int)(__float_as_uint(top) >> 23) - 126, -100); }  // top < 2^R
+__device__ __forceinline__ int up_R(float v_up) { return 14 + 127 - (int)(__float_as_uint(v_up) >> 23); }         // 2^(14 - R)
+__device__ __forceinline__ bool scale_fits(float size, int R) {
+    return size == 0.f || (size >= exp2i(R - 16) && size <= exp2i(min(R + 1, 127)));
+}
+template <int NG>
+__device__ __forceinline__ void set_low(uint32_t& v_low, int gr, int R) {
+    const uint32_t low = 0x10000u - (uint32_t)((R - 16 + 127) << 7), in_gr = NG == 1 ? 0xffffffffu : 0xffffu << 16 * gr;
+    v_low = (v_low & ~in_gr) | (low * 0x10001u & in_gr);
+}
+
+// A step with scales of V that f16 does not hold together with the others: R
+// moves where none of the step's fits any more, the sums are scaled to it, and
+// the keys that still do not fit are added to the sums one by one in f32 and
+// their scales zeroed.  All 32 lanes call it with what they hold of the step;
+// a function of its own, since the registers of the kernel's loop are full.
+template <int NT, int NG>
+struct FarScales {
+    float o[NT][NG][4][4], vs[2][2][NG], p[2][2][NT][2], v_up[NG];
+    uint32_t v_low;
+};
+template <int D, int NT>
+__device__ __noinline__ void far_scales(FarScales<NT, D / KV4_GROUP>& k, uint32_t v_stage) {
+    constexpr int NG = D / KV4_GROUP, MT = 4;
+    const int lane = threadIdx.x & 31, g = lane >> 2, c = lane & 3;
+#pragma unroll 1
+    for (int gr = 0; gr < NG; gr++) {
+        int R = up_R(k.v_up[gr]);
+        float top = 0.f;
+        bool any = false;
+        for (int hr = 0; hr < 4; hr++) {
+            const float y = scale_size(k.vs[hr >> 1][hr & 1][gr]);
+            top = fmaxf(top, y);
+            any = any || (y > 0.f && scale_fits(y, R));
+        }
+        top = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top)));
+        if (top == 0.f) continue;
+        int to = R;
+        if (!__any_sync(0xffffffffu, any)) {
+            const int Rt = scale_R(top);
+            if (Rt > R) {
+                if (Rt <= R + 60) to = Rt;  // (more would leave nothing of the sums so far)
+            } else {
+                // down, as far as the sums so far stay within f32
+                float big = 0.f;
+                for (int nt = 0; nt < NT; nt++)
+                    for (int i = 0; i < 4 * MT; i++) big = fmaxf(big, fabsf(k.o[nt][gr][i / 4][i % 4]));
+                big = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(big)));
+                to = max(Rt, R - min(max(120 + 127 - (int)(__float_as_uint(big) >> 23), 0), 120));
+            }
+        }
+        to = max(to, scale_R(top) - 110);  // (the largest scale times 2^(14 - R) stays within f32)
+        const float f = exp2i(max(R - to, -126)), up = exp2i(14 - to);
+        R = to;
+        k.v_up[gr] = up;
+        set_low<NG>(k.v_low, gr, R);
+        for (int nt = 0; nt < NT; nt++)
+            for (int i = 0; i < 4 * MT; i++) k.o[nt][gr][i / 4][i % 4] *= f;
+#pragma unroll 1
+        for (int hr = 0; hr < 4; hr++) {
+            const int h = hr >> 1, r = hr & 1;
+            const float scaled = k.vs[h][r][gr] * up * 0x1p-24f;
+            const bool out = !scale_fits(scale_size(k.vs[h][r][gr]), R);
+            if (out) k.vs[h][r][gr] = 0.f;
+            unsigned left = __ballot_sync(0xffffffffu, out && c == 0);
+#pragma unroll 1
+            while (left) {
+                const int src = __ffs(left) - 1, gk = src >> 2;
+                left &= left - 1;
+                const float sk = __shfl_sync(0xffffffffu, scaled, src);
+                const uint32_t w = lds32(v_stage + stage_at<D>(16 * h + 8 * r + (gk >> 1) + 4 * (gk & 1), gr * 32 + g * 4));
+                for (int nt = 0; nt < NT; nt++)
+                    for (int j = 0; j < 2; j++) {
+                        const float p = __shfl_sync(0xffffffffu, k.p[h][r][nt][j], src + c), ps = p == 0.f ? 0.f : p * sk;
+                        for (int t = 0; t < MT; t++) {
+                            k.o[nt][gr][t][j] = fmaf(ps, (float)(w >> 8 * t & 15), k.o[nt][gr][t][j]);
+                            k.o[nt][gr][t][2 + j] = fmaf(ps, (float)(w >> (8 * t + 4) & 15) * 16.f, k.o[nt][gr][t][2 + j]);
+                        }
+                    }
+            }
+        }
+    }
+}
+
 template <int D, int NT>
 __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(const __grid_constant__ Kv4Attend a) {
     using C = AttnCfg<D, NT>;
@@ -196,6 +298,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
     v_off[0] = C::VAL + stage_at<D>(c, g * 4);
     v_off[1] = C::VAL + stage_at<D>(c + 4, g * 4) - 4 * C::ROW;
     const uint32_t p_off = 2 * C::VAL + ((g >> 1) + 4 * (g & 1)) * (NG * 4);
+    const uint32_t v_own = C::PAR + 8 * c * (NG * 4);  // from there: V's parameters of the one of the lane's four keys that it checks
 
     griddep_wait();
     griddep_launch_dependents();
@@ -345,12 +448,12 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
         const int all_hi = min(min_hi, k1);
 
         float m[NT][2], l[NT][2], zs[NT][NG][2], o[NT][NG][MT][4];
-        float v_up[NG], v_lim[NG];  // 2^(14 - R), 2^(R + 1)
+        // Per group: 2^(14 - R), and (group 0 in the low half) less the smallest scale that f16 holds with it, as bf16
+        // bits; no scale fits before the first is met.
+        float v_up[NG];
+        uint32_t v_low = V_UNSET;
 #pragma unroll
-        for (int gr = 0; gr < NG; gr++) {
-            v_up[gr] = 1.f;
-            v_lim[gr] = -1.f;
-        }
+        for (int gr = 0; gr < NG; gr++) v_up[gr] = 1.f;
 #pragma unroll
         for (int nt = 0; nt < NT; nt++) {
 #pragma unroll
@@ -383,6 +486,16 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
             stage = stage + 1 == C::STAGES ? 0 : stage + 1;
             const int key0 = k0 + (i * AT_WARPS + warp) * AT_STEP;
             const bool edge = key0 + AT_STEP > all_hi || key0 < max_lo;
+            // whether a scale of V leaves f16's reach: a lane looks at one key's, all of its groups at once
+            uint32_t scales;
+            if constexpr (NG == 2) {
+                const uint2 t = lds64(p_at + v_own);
+                scales = __byte_perm(t.x, t.y, 0x5410);
+            } else {
+                scales = lds32(p_at + v_own) & 0xffffu;
+                scales |= scales << 16;
+            }
+            const bool far = scales != 0 && umax2(uadd2(scales, v_low), V_SPAN) != V_SPAN;
             float x[2][NT][4];  // [16 keys][columns][C fragment]: S, then P
             float vs[2][2][NG], vz[2][2][NG];
 #pragma unroll
@@ -507,28 +620,77 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
             }
 
             // ---- V's scales within f16's reach
-            float top[NG];
-            bool over = false;
-#pragma unroll
-            for (int gr = 0; gr < NG; gr++) {
-                top[gr] = fmaxf(fmaxf(fabsf(vs[0][0][gr]), fabsf(vs[0][1][gr])), fmaxf(fabsf(vs[1][0][gr]), fabsf(vs[1][1][gr])));
-                over = over || top[gr] > v_lim[gr];
-            }
-            if (__any_sync(0xffffffffu, over)) {
+            bool cold = false;
+            if (__any_sync(0xffffffffu, far)) {
+                // The first ones, or a little more than before: R rises.  (Or only a scale of zero or of another sign,
+                // or a key that no row sees.)
+                const int own = key0 + 8 * c + (g >> 1) + 4 * (g & 1);
+                uint32_t mine = own < k1 && own >= p.kr.first ? scales & 0x7fff7fffu : 0u;
 #pragma unroll
                 for (int gr = 0; gr < NG; gr++) {
-                    const float most = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(top[gr])));
-                    if (!(most > v_lim[gr])) continue;
-                    const int R = max((int)(__float_as_uint(most) >> 23) - 126, -100);  // most < 2^R
-                    const float up = exp2i(14 - R), f = up / v_up[gr];
-                    v_lim[gr] = exp2i(min(R + 1, 127));
-                    v_up[gr] = up;
+                    if ((mine >> 16 * gr & 0xffffu) >= 0x7f80u) mine &= NG == 1 ? 0u : gr ? 0x0000ffffu : 0xffff0000u;  // not finite
+                    const int top = __reduce_max_sync(0xffffffffu, mine >> 16 * gr & 0xffffu);
+                    const bool unset = (v_low >> 16 * gr & 0xffffu) == (V_UNSET & 0xffffu);
+                    const int R = max((top >> 7) - 126, -100), R0 = up_R(v_up[gr]);
+                    if (top == 0 || !(unset || (R > R0 + 1 && R <= R0 + 9))) continue;
+                    const float f = unset ? 0.f : exp2i(R0 - R);
+                    v_up[gr] = exp2i(14 - R);
+                    set_low<NG>(v_low, gr, R);
 #pragma unroll
                     for (int nt = 0; nt < NT; nt++)
 #pragma unroll
                         for (int t = 0; t < MT; t++)
 #pragma unroll
                             for (int i4 = 0; i4 < 4; i4++) o[nt][gr][t][i4] *= f;
+                }
+                const uint32_t off = umax2(uadd2(mine, v_low), V_SPAN) ^ V_SPAN;
+                cold = ((mine & 0xffffu) && (off & 0xffffu)) || ((mine >> 16) && (off >> 16));
+                cold = __any_sync(0xffffffffu, cold);
+            }
+            if (cold) {
+                FarScales<NT, NG> k;
+                k.v_low = v_low;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    k.v_up[gr] = v_up[gr];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) k.vs[h][r][gr] = vs[h][r][gr];
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; nt++) {
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) {
+                            float y[2];
+                            upk2(mul2(add2(pk2(x[h][nt][2 * r], x[h][nt][2 * r + 1]), less[nt]), by[nt]), y[0], y[1]);
+                            k.p[h][r][nt][0] = ex2(y[0]);
+                            k.p[h][r][nt][1] = ex2(y[1]);
+                        }
+#pragma unroll
+                    for (int gr = 0; gr < NG; gr++)
+#pragma unroll
+                        for (int t = 0; t < MT; t++)
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; i4++) k.o[nt][gr][t][i4] = o[nt][gr][t][i4];
+                }
+                far_scales<D, NT>(k, st + C::VAL);
+                v_low = k.v_low;
+#pragma unroll
+                for (int gr = 0; gr < NG; gr++) {
+                    v_up[gr] = k.v_up[gr];
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+#pragma unroll
+                        for (int r = 0; r < 2; r++) vs[h][r][gr] = k.vs[h][r][gr];
+#pragma unroll
+                    for (int nt = 0; nt < NT; nt++)
+#pragma unroll
+                        for (int t = 0; t < MT; t++)
+#pragma unroll
+                            for (int i4 = 0; i4 < 4; i4++) o[nt][gr][t][i4] = k.o[nt][gr][t][i4];
                 }
             }
 
@@ -591,7 +753,7 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
             for (int gr = 0; gr < NG; gr++) {
                 float z[2];
-                const float back = 1.f / v_up[gr];  // 2^(R - 14)
+                const float back = 1.f / v_up[gr];  // 2^(R - 14), before the rest, so that nothing passes f32 on the way
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
                     z[j] = zs[nt][gr][j];
@@ -603,8 +765,8 @@ __global__ void __launch_bounds__(AT_WARPS * 32, NT == 1 ? 2 : 1) sp_kv4_attend(
 #pragma unroll
                     for (int r = 0; r < 2; r++)
                         *(float2*)(sm_o + ((nt * NG + gr) * 64 + (2 * t + r) * 8 + g) * 8 + 2 * c) =
-                            make_float2(fmaf(o[nt][gr][t][2 * r] * (r ? 0x1p20f : 0x1p24f), back, z[0]),
-                                        fmaf(o[nt][gr][t][2 * r + 1] * (r ? 0x1p20f : 0x1p24f), back, z[1]));
+                            make_float2(fmaf(o[nt][gr][t][2 * r] * back, r ? 0x1p20f : 0x1p24f, z[0]),
+                                        fmaf(o[nt][gr][t][2 * r + 1] * back, r ? 0x1p20f : 0x1p24f, z[1]));
             }
 #pragma unroll
             for (int j = 0; j < 2; j++) {

@@ -1108,3 +1108,30 @@ def test_attend_scales_of_either_sign(engines, d, rows):
     b.attend(engines[d], engines["ws", d])
     check_attend(b, "signs")
     engines[d].engine_status()
+
+
+def huge_values(engines, d, size, rows):
+    """A cached V far beyond the others', seen by the later half of the queries only, and one that all see whose
+    probability is nothing: the other rows keep their precision, and the rows that see it stay finite."""
+    n = 700
+    b = Batch(d, 32, 4, 2, [n, 60], [rows, 1], seed=rows + d, tail_rows=0)
+    hidden = n - rows + rows // 2
+    b.v[hidden] *= size
+    b.v[n - rows - 9, 1, 5] = size  # one channel only: its group's other values are lost in its scale
+    b.v[200] *= size
+    for h in range(2):
+        u = torch.randn(d, generator=gen(h), device=DEV)
+        b.q[:rows, 2 * h:2 * h + 2] = (u + 0.3 * b.q[:rows, 2 * h:2 * h + 2].float()).bfloat16()
+        b.k[200, h] = (-30 * u).bfloat16()  # a score far below the others'
+        b.k[n - rows - 9, h] = (-30 * u).bfloat16()
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    check_attend(b, "V")
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e20, 1e30, 1e32, 2e37])
+@pytest.mark.parametrize("rows", [3, 5, 40])
+def test_attend_huge_finite_values_stay_with_the_rows_that_see_them(engines, d, size, rows):
+    huge_values(engines, d, size, rows)
