@@ -592,9 +592,13 @@ typedef struct {
  * sees no key gives zeros and an lse of -infinity.  q is bf16 and already
  * rotated; K and V are the cached values, scores and lse those of the exact
  * ones to f32's rounding, sums f32; a probability times its V scale is rounded
- * to f16 (2^-11).  With max_q * heads / kv_heads above 128 (prompts) each V
- * value and each probability is, and K scales more than 2^8 apart within 128
- * keys are rounded by 2^-16 of the largest.  opts: the softmax scale (default
+ * to f16 (2^-11; below 2^-26 of the row's largest nothing may be left of it).  With
+ * max_q * heads / kv_heads above 128 (prompts) each V value and each probability
+ * is (a value by 2^-10 of the largest that its group's scale can give where it
+ * is small, a probability below 2^-28 counts as 0), and where the scales of one
+ * key's two groups of K are more than 2^8 apart, the smaller one's products are
+ * rounded by 2^-17 of the larger scale.  A row's precision depends on the keys
+ * that it sees alone.  opts: the softmax scale (default
  * 1 / sqrt(head_dim)) is taken, the smoothing flags are not, a QK LayerNorm is
  * refused; NULL = default.  The scale must lie in 1e-10 .. 1e10.  out must not
  * overlap q; rows of no sequence are left as they were.  lse: f32

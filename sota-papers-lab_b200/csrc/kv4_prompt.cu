@@ -11,6 +11,7 @@
 //               time.  While A's scores are worked on, the tensor core
 //               computes B's, and the other way round.
 //   warps 8-15  unpack the next tile into shared memory
+//   warp 17     unpacks a tile whose keys' magnitudes are far apart, in turns
 //   warp 16     one thread issues tcgen05.mma: S = Q K^T (f16, both operands
 //               from shared memory, S in TMEM) and O += P V (f16, P from
 //               TMEM, where it takes the place of its S)
@@ -18,18 +19,18 @@
 // of both (D columns each).
 //
 // K: scale * (n - 8) has 8 + 3 significant bits, so it is EXACT in f16 when
-// scaled by a power of two 2^-E (one for the tile: the products of scales below
-// a 2^-8 of the tile's largest are rounded by 2^-16 of the largest); the rest
-// of the value, c = zero + 8 scale, is constant per group of 64 channels and
-// enters through 16 more channels, as two f16 terms times two f16 terms of the
-// row's sum over the group (an error below 2^-20 of that product).  So S is
-// that of the exact cached values to f32's rounding, and lse with it, where
-// f16 values of K would put a row's lse off by 1e-4 and more.
-// V: zero + scale * n rounded to f16 (2^-11 of itself at most, 2^-21 of the
-// tile's largest), scaled per tile by a power of two 2^-R; P, times 2^7 and
-// what R differs from the largest R so far, rounded to f16 likewise; sums in
-// f32.  (bf16 for both, which needs no R, left the output off by 0.0028 of
-// itself against 64 bits instead of 0.0017, and unpacked slower.)
+// scaled by a power of two 2^-E; the rest of the value, c = zero + 8 scale, is
+// constant per group of 64 channels and enters through 16 more channels, as two
+// f16 terms times two f16 terms of the row's sum over the group (an error below
+// 2^-20 of that product).  So S is that of the exact cached values to f32's
+// rounding, and lse with it, where f16 values of K would put a row's lse off by
+// 1e-4 and more.  Each row of Q is scaled by a power of two of its own.
+// V: zero + scale * n, scaled by a power of two 2^-R, rounded to f16 (2^-11 of
+// itself, or 2^-25 of 2^R where that is more); P, times 2^7 and what R differs
+// from the R that the row's O refers to, rounded to f16 likewise; sums in f32.
+// (bf16 for both, which needs no R, left the output off by 0.0028 of itself
+// against 64 bits instead of 0.0017, and unpacked slower.)
+// E and R hold for the keys of a tile that share them: see K_WIDE.
 //
 // The running maximum a row's exponents refer to is only raised when a new one
 // is more than 2^8 larger (P and the sums have room for that), so O is hardly
@@ -52,8 +53,9 @@ namespace sp {
 
 constexpr int PR_ROWS = 256, PR_KEYS = 128;
 constexpr int PR_LEAST = 4;  // key tiles a CTA takes at least: a piece's start, end and joining cost as much as several
+constexpr uint32_t R_BELOW = 4;  // how far a tile's R may lie below the one that a row's O refers to: P of 2^-28 is not lost
 constexpr int PR_BEGIN = 3;  // what a tile's start and end count for when they are shared out (549 us instead of 575, 551 with 6)
-constexpr int PR_SOFTMAX = 8, PR_UNPACK = 8, PR_MMA_WARP = 16, PR_THREADS = 20 * 32;
+constexpr int PR_SOFTMAX = 8, PR_UNPACK = 8, PR_MMA_WARP = 16, PR_HELP_WARP = 17, PR_THREADS = 20 * 32;
 // Registers a thread: what the block is launched with, and what the
 // warpgroups make of them (raising more than there are would wait for ever).
 constexpr int PR_REGS = 96, PR_REGS_SOFTMAX = 128, PR_REGS_UNPACK = 88, PR_REGS_MMA = 48;
@@ -131,6 +133,9 @@ __device__ __forceinline__ uint32_t hfma2(uint32_t a, uint32_t b, uint32_t c) {
 __device__ __forceinline__ void sts128(uint32_t p, uint32_t a, uint32_t b, uint32_t c, uint32_t d) {
     asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(p), "r"(a), "r"(b), "r"(c), "r"(d) : "memory");
 }
+__device__ __forceinline__ void sts16(uint32_t p, uint32_t v) {
+    asm volatile("st.shared.b16 [%0], %1;" ::"r"(p), "h"((uint16_t)v) : "memory");
+}
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -140,17 +145,248 @@ __device__ __forceinline__ float max3(float a, float b, float c) {
     asm("max.f32 %0, %1, %2, %3;" : "=f"(r) : "f"(a), "f"(b), "f"(c));
     return r;
 }
-// Element-wise maxima of two 16-bit halves.
+// Element-wise maxima and sums of two 16-bit halves.
 __device__ __forceinline__ uint32_t umax2(uint32_t a, uint32_t b) {
     uint32_t d;
     asm("max.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
     return d;
+}
+__device__ __forceinline__ uint32_t uadd2(uint32_t a, uint32_t b) {
+    uint32_t d;
+    asm("add.u16x2 %0, %1, %2;" : "=r"(d) : "r"(a), "r"(b));
+    return d;
+}
+// A named barrier that says whether any of its threads came with `x`.
+__device__ __forceinline__ bool named_bar_any(uint32_t id, uint32_t count, bool x) {
+    uint32_t r;
+    asm volatile(
+        "{\n .reg .pred p, q;\n setp.ne.b32 q, %3, 0;\n bar.red.or.pred p, %1, %2, q;\n selp.u32 %0, 1, 0, p;\n}"
+        : "=r"(r)
+        : "r"(id), "r"(count), "r"((uint32_t)x)
+        : "memory");
+    return r != 0;
 }
 __device__ __forceinline__ int bexpo(uint32_t bf16_bits) { return (int)(bf16_bits >> 7 & 255) - 127; }
 // x as two f16 terms, (hi, lo) in one word
 __device__ __forceinline__ uint32_t split_half(float x) {
     const __half hi = __float2half_rn(x);
     return half2_bits(__half2float(hi), x - __half2float(hi));
+}
+
+// A turn of a tile: what its K and V were scaled by (2^-E, 2^-R), whether
+// another turn of the same tile follows, and whether its keys have been counted
+// in the rows' sums by an earlier one.
+struct __align__(16) PromptTile {
+    int E, R;
+    uint32_t more, again;
+};
+
+// E and R stay the same from tile to tile as long as all keys' scales fit them:
+// K's from 2^-K_WIDE of the largest that f16 holds with E on (its products are
+// exact then: 8 bits of scale, 3 of n - 8 above f16's 2^-24), V's from
+// 2^-V_WIDE (its values are off by 2^-10 of the largest that the smallest such
+// scale can give).  Any other tile goes to the helper, which finds E and R for
+// it; where its keys are too far apart for one pair, or not finite, it works on
+// the tile in turns, each with the keys whose magnitudes go together and all
+// others hidden, so that no key takes precision from the rows that do not see it.
+constexpr int K_WIDE = 8, V_WIDE = 10;
+// E and R for a scale and zero (bf16 bits, zero in the upper half).  K: scales
+// below 2^-8, c below 2^6; V: scales below 2^-8, zeros below 2^13.
+__device__ __forceinline__ int key_E(uint32_t k) { return min(max(max(bexpo(k) + 9, bexpo(k >> 16) - 4), -100), 136); }
+__device__ __forceinline__ int key_R(uint32_t v) { return min(max(max(bexpo(v) + 9, bexpo(v >> 16) - 12), -100), 136); }
+__device__ __forceinline__ bool finite2(uint32_t p) { return (p & 0x7f80u) != 0x7f80u && (p & 0x7f800000u) != 0x7f800000u; }
+// Where the scales and zeros that fit lie, as bf16 bits: with x added to them
+// (half by half), at most y.
+__device__ __forceinline__ uint2 fitting(int most_scale, int least_scale, int most_zero) {
+    auto bits = [](int e) { return (uint32_t)min(max(e + 127, 1), 255) << 7; };  // of 2^e
+    const uint32_t low = bits(least_scale);
+    return make_uint2(0x10000u - low, (min(bits(most_zero + 1) - 1, 0x7f7fu) << 16) | (min(bits(most_scale + 1) - 1, 0x7f7fu) - low));
+}
+
+// What the unpacking warps and the helper share.
+struct FarTile {
+    uint4 fit;  // what fits E and R: K's x and y, V's
+    int E, R;
+    uint32_t kp[2][PR_KEYS], vp[2][PR_KEYS];  // the tile's keys' parameters by group (0: not wanted)
+    uint32_t keys[4], values[2][4];           // the turn's keys, a bit each; those of them with V, by group
+    int tile0, end;                           // its first key; that behind its last
+    uint32_t t, marks;                        // the next turn; K's stages that hold marks of hidden keys, a bit each
+    int piece;                                // -1: no more tiles
+    bool set, done, ok;                       // E and R are; the helper did all of the tile; no wait ran out
+};
+
+// Picks the keys of a tile's turn `pass` (a warp calls it): of those that no
+// earlier turn took, the ones whose own E is within K_WIDE of the largest, and
+// of these the ones with a group of V whose own R is within V_WIDE of the
+// largest (so at least one each time), with those groups.  Once all keys have
+// had a turn, the same for the groups that are left of them.  A K or V of zero,
+// and one that is not finite, fits any.  Returns whether the tile takes more
+// than plain unpacking.
+__device__ __forceinline__ bool pick_keys(PromptTile& tile, FarTile& far, int groups, int pass) {
+    const int lane = threadIdx.x & 31;
+    constexpr int ANY = -1000;
+    int E[4], R[4][2];
+    bool bad = false;
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        E[b] = R[b][0] = R[b][1] = ANY;
+#pragma unroll
+        for (int gr = 0; gr < 2; gr++) {
+            if (gr >= groups) break;
+            const uint32_t k = far.kp[gr][32 * b + lane] & 0x7fff7fffu, v = far.vp[gr][32 * b + lane] & 0x7fff7fffu;
+            if (k && finite2(k)) E[b] = max(E[b], key_E(k));
+            if (v && finite2(v)) R[b][gr] = key_R(v);
+            bad = bad || !finite2(v);
+        }
+    }
+    // Of the lane's four keys, a bit each: those without a turn so far, those with group 0 or 1 of V left, and the turn's
+    uint32_t fresh = 15, left[2] = {15, groups == 2 ? 15u : 0u}, now = 0, with[2] = {0, 0};
+    int top_E = 0, top_R = 0;
+    bool first = true;
+#pragma unroll 1
+    for (int i = 0; i <= pass; i++) {
+        fresh &= ~now;
+        left[0] &= ~with[0];
+        left[1] &= ~with[1];
+        first = __any_sync(0xffffffffu, fresh);
+        const uint32_t open = first ? fresh : left[0] | left[1];
+        uint32_t near = 0;
+        int top = ANY;
+#pragma unroll
+        for (int b = 0; b < 4; b++) top = max(top, open >> b & 1 ? E[b] : ANY);
+        top_E = max(__reduce_max_sync(0xffffffffu, top), -100);
+        if (far.set && far.E > top_E && far.E <= top_E + 2) top_E = far.E;  // (no need to go up and down)
+        top = ANY;
+#pragma unroll
+        for (int b = 0; b < 4; b++)
+            if ((open >> b & 1) && (E[b] == ANY || E[b] >= top_E - K_WIDE)) {
+                near |= 1u << b;
+#pragma unroll
+                for (int gr = 0; gr < 2; gr++)
+                    if (left[gr] >> b & 1) top = max(top, R[b][gr]);
+            }
+        top_R = max(__reduce_max_sync(0xffffffffu, top), -100);
+        if (far.set && far.R > top_R && far.R <= top_R + 2) top_R = far.R;
+#pragma unroll
+        for (int gr = 0; gr < 2; gr++) {
+            with[gr] = 0;
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                if ((near & left[gr]) >> b & 1 && (R[b][gr] == ANY || R[b][gr] >= top_R - V_WIDE)) with[gr] |= 1u << b;
+        }
+        now = with[0] | with[1];
+    }
+    const uint32_t behind = (fresh & ~now) | (left[0] & ~with[0]) | (left[1] & ~with[1]);
+    const bool more = __any_sync(0xffffffffu, behind);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const uint32_t word = __ballot_sync(0xffffffffu, now >> b & 1), v0 = __ballot_sync(0xffffffffu, with[0] >> b & 1),
+                       v1 = __ballot_sync(0xffffffffu, with[1] >> b & 1);
+        if (lane == 0) {
+            far.keys[b] = word;
+            far.values[0][b] = v0;
+            far.values[1][b] = v1;
+        }
+    }
+    if (lane == 0) {
+        tile.E = top_E;
+        tile.R = top_R;
+        tile.more = more;
+        tile.again = !first;
+    }
+    return __any_sync(0xffffffffu, bad || behind || now != 15);
+}
+
+// K's values of one key and group, scaled by 2^-E: scale * (n - 8) in f16.
+struct K4 {
+    uint32_t sl, sh, off;
+    __device__ __forceinline__ K4(uint32_t kp, int E) {
+        const float s24 = __uint_as_float(kp << 16) * exp2i(24 - E), m8 = s24 * -0x1p-21f;
+        sl = half2_bits(s24, s24);
+        sh = half2_bits(s24 * 0x1p-4f, s24 * 0x1p-4f);
+        off = half2_bits(m8, m8);
+    }
+    __device__ __forceinline__ void put(uint32_t dst, uint32_t lo) const {  // 8 channels
+        const uint32_t hi = lo >> 8;
+        sts128(dst, hfma2(lo & 0x000f000fu, sl, off), hfma2(lo & 0x00f000f0u, sh, off), hfma2(hi & 0x000f000fu, sl, off),
+               hfma2(hi & 0x00f000f0u, sh, off));
+    }
+    // c = zero + 8 scale as two terms
+    static __device__ __forceinline__ uint32_t extra(uint32_t kp, int E) {
+        return split_half(fmaf(8.f, __uint_as_float(kp << 16), __uint_as_float(kp & 0xffff0000u)) * exp2i(24 - E) * 0x1p-16f);
+    }
+};
+// A key's 16 more channels: (hi, hi, lo, lo) of each group, against the row's (hi, lo, hi, lo)
+template <int D>
+__device__ __forceinline__ void put_extra(uint32_t base, uint32_t st, int kk, const uint32_t (&cw)[2]) {
+    using C = PromptCfg<D>;
+    sts128(base + C::KX_OFF + st * C::X + kk * 32 + ((kk >> 2 & 1) << 4), __byte_perm(cw[0], 0, 0x1010),
+           __byte_perm(cw[0], 0, 0x3232), __byte_perm(cw[1], 0, 0x1010), __byte_perm(cw[1], 0, 0x3232));
+}
+// A thread's part of K's stage: half of a key's channels (D = 128: a group), and the 16 more.
+template <int D>
+__device__ __forceinline__ void put_k(uint32_t base, uint32_t st, int kk, int kh, const uint32_t (&kw)[D / 16],
+                                      const uint32_t (&kp)[D / KV4_GROUP], int E) {
+    using C = PromptCfg<D>;
+    constexpr int NG = C::NG, KW = D / 16;
+    const K4 k(kh == 0 ? kp[0] : kp[NG - 1], E);
+    const uint32_t dst = base + C::K_OFF + st * C::K + (NG == 2 ? kh * C::ATOM : 0) + kk * 128 + ((kk & 7) << 4);
+#pragma unroll
+    for (int i = 0; i < KW; i++) k.put(dst ^ ((NG == 2 ? i : kh * KW + i) << 4), kw[i]);
+    if (kh == 0) {
+        uint32_t cw[2] = {0, 0};
+#pragma unroll
+        for (int gr = 0; gr < NG; gr++) cw[gr] = K4::extra(kp[gr], E);
+        put_extra<D>(base, st, kk, cw);
+    }
+}
+
+// ... and of V's: 8 channels of 8 keys (finite ones), scaled by 2^-R.
+template <int D>
+__device__ __forceinline__ void put_v(uint32_t base, uint8_t* sm, uint32_t st, uint32_t t, int vk, int vc,
+                                      const uint32_t (&vw)[8], const uint32_t (&vp)[8], int R) {
+    using C = PromptCfg<D>;
+    const float up = exp2i(24 - R);
+    uint32_t sl[4], sh_[4], ze[4];  // of two keys: scale * 2^24 and 2^20, zero, times 2^-R
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const uint32_t p0 = vp[2 * i], p1 = vp[2 * i + 1];
+        const float s0 = __uint_as_float(p0 << 16) * up, s1 = __uint_as_float(p1 << 16) * up;
+        sl[i] = half2_bits(s0, s1);
+        sh_[i] = half2_bits(s0 * 0x1p-4f, s1 * 0x1p-4f);
+        ze[i] = half2_bits(__uint_as_float(p0 & 0xffff0000u) * up * 0x1p-24f, __uint_as_float(p1 & 0xffff0000u) * up * 0x1p-24f);
+    }
+    if ((vc & 7) == 0) sm[C::N_OFF + (t & 3) * 32 + vc / 8 * 16 + vk] = 0;
+    const uint32_t dst = base + C::V_OFF + st * C::V + (vk >> 3) * (D * 128) + vc * 1024 + ((vk & 7) << 4);
+#pragma unroll
+    for (int b = 0; b < 4; b++) {
+        const uint32_t sel = b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12);
+        uint32_t lo[4], hi[4];
+#pragma unroll
+        for (int i = 0; i < 4; i++) {
+            const uint32_t y = __byte_perm(vw[2 * i], vw[2 * i + 1], sel);
+            lo[i] = hfma2(y & 0x000f000fu, sl[i], ze[i]);
+            hi[i] = hfma2(y & 0x00f000f0u, sh_[i], ze[i]);
+        }
+        const int r0 = 2 * b, r1 = 2 * b + 1;  // channels 8 vc + r
+        sts128((dst ^ (r0 << 4)) + r0 * 128, lo[0], lo[1], lo[2], lo[3]);
+        sts128((dst ^ (r1 << 4)) + r1 * 128, hi[0], hi[1], hi[2], hi[3]);
+    }
+}
+
+// The largest magnitude of a row of O.
+template <int D>
+__device__ __forceinline__ float most_of(uint32_t tm_o) {
+    float most = 0.f;
+#pragma unroll 1
+    for (int ch = 0; ch < D / 32; ch++) {
+        uint32_t y[32];
+        tmem_ld32(tm_o + 32 * ch, y);
+        tmem_wait_ld();
+#pragma unroll
+        for (int i = 0; i < 32; i++) most = fmaxf(most, fabsf(__uint_as_float(y[i])));
+    }
+    return most;
 }
 
 template <int D>
@@ -168,10 +404,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
     // key tiles (so two pieces) ahead of the softmax.
     __shared__ Piece pieces[RING];
     __shared__ int8_t sm_up[PR_ROWS];  // the power of two that each row of Q was scaled by
-    // The largest scales and zeros of a tile, as bf16 bits (zero in the upper half), of each unpacking warp's part
-    __shared__ uint2 sm_top[2][PR_UNPACK];
-    __shared__ int sm_E[4];  // of a tile: its K was scaled by 2^-E
-    __shared__ int sm_R[4];  // ... and its V by 2^-R
+    __shared__ PromptTile sm_tile[4];
+    __shared__ FarTile sm_far;
+    __shared__ uint32_t sm_t;  // turns that A has worked on
     __shared__ float2 sm_join[PR_SOFTMAX * 32 / (D / 4)];
     __shared__ bool sm_last;
     __shared__ volatile uint32_t sm_gave_up;  // a wait of this CTA ran out
@@ -183,7 +418,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
     uint8_t* const sm = dyn_smem + (base - smem_u32(dyn_smem));
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     auto bar = [&](uint64_t& b) { return smem_u32(&b); };
-    if (tid == 0) sm_gave_up = 0;
+    if (tid == 0) {
+        sm_gave_up = 0;
+        sm_far.fit = make_uint4(0x8000u, 0u, 0x8000u, 0u);  // nothing fits
+        sm_far.set = false;
+    }
 
     griddep_wait();
     if (blockIdx.x == 0)  // what is out of range is reported once
@@ -214,10 +453,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
         mbar_init(bar(bars.drained), 1);
         fence_barrier_init();
     }
-    // the second half of the extra channels' rows stays zero
+    // the second half of the extra channels' rows: Q's first is 1 (against K's, which hides a key with -infinity there),
+    // the rest zero
     for (int i = tid; i < 4 * 128; i += PR_THREADS) {
         const int row = i & 127;
-        *(uint4*)(sm + C::QX_OFF + (i >> 7) * C::X + row * 32 + ((1 ^ (row >> 2 & 1)) << 4)) = make_uint4(0, 0, 0, 0);
+        *(uint4*)(sm + C::QX_OFF + (i >> 7) * C::X + row * 32 + ((1 ^ (row >> 2 & 1)) << 4)) = make_uint4(i < 256 ? 0x3c00u : 0u, 0, 0, 0);
     }
     __syncthreads();
     if (!pieces[0].any) return;
@@ -240,7 +480,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
         const int x = warp >> 2, row = (warp & 3) * 32 + lane;
         const uint32_t lanes = (uint32_t)(warp & 3) << 21;  // TMEM lane base in the address
         const uint32_t tm_s = tmem + 128 * x + lanes, tm_o = tmem + 256 + D * x + lanes;
-        uint32_t t = 0, tx = 0, rounds = 0, events = 0;  // key tiles so far, those that A (B) worked on, pieces it worked on
+        // Turns of key tiles so far, those that A (B) worked on, pieces it worked on
+        uint32_t t = 0, tx = 0, rounds = 0, events = 0;
         for (int turn = 0;; turn++) {
             const Piece& p = pieces[turn % RING];
             const Seq s = p.at.s;
@@ -316,9 +557,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 const bool live = __any_sync(0xffffffffu, nr < rows);
                 const bool leader = (warp & 3) == 0;
                 bool all_ok = true;  // of the group's four warps
-                // V of tile j that is not finite reaches the rows that see the key.
+                // V of the last turn (of tile j) that is not finite reaches the rows that see the key.
                 auto see_bad = [&](int j) {
-                    const uint4* bad = (const uint4*)(sm + C::N_OFF + ((t + j) & 3) * 32);
+                    const uint4* bad = (const uint4*)(sm + C::N_OFF + ((t - 1) & 3) * 32);
 #pragma unroll
                     for (int gr = 0; gr < NG; gr++) {
                         const uint4 b = bad[gr];
@@ -332,19 +573,22 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         }
                     }
                 };
-                for (int j = 0; j < n; j++) {
-                    const uint32_t tj = t + j;
+                int last = 0;  // the tile of the turn before
+                bool first = true;
+                for (int j = 0; j < n;) {
+                    const uint32_t tj = t;
                     // One warp of the four waits (each poll costs issue slots), the others at a barrier.
                     if (leader)
                         sm_go[x][events & 1] = warp_all_wait(bar(bars.f_full[tj & 3]), tj >> 2 & 1, a.err, 61) &&
-                                               warp_all_wait(bar(bars.s_full[x]), (tx + j) & 1, a.err, 60) && !sm_gave_up;
+                                               warp_all_wait(bar(bars.s_full[x]), tx & 1, a.err, 60) && !sm_gave_up;
                     named_bar(4 + x, PR_SOFTMAX * 16);
                     all_ok = sm_go[x][events++ & 1];
                     if (!all_ok) break;
                     ok = true;
-                    if (j > 0) see_bad(j - 1);
+                    if (!first) see_bad(last);
                     tc_fence_after();
                     const int key0 = k0 + j * PR_KEYS;
+                    const PromptTile tile = sm_tile[tj & 3];
                     auto hand_over = [&](int h) {
                         tc_fence_before();
                         __syncwarp();
@@ -352,10 +596,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     };
                     if (live) {
                         const bool edge = key0 + PR_KEYS > all_hi || key0 < all_lo;
-                        const int R = sm_R[tj & 3];
-                        bool raise = j == 0 || R > R_ref;  // (the same in all rows)
+                        const int R = tile.R;
+                        if (first) R_ref = R + 2;
+                        bool far_R = (uint32_t)(R_ref - R) > R_BELOW;
+                        // (at most 7, so P at most 2^15; below -40 nothing is left of it in f16)
+                        int shift = min(max(7 + R - R_ref, -40), 7);
                         // what S is multiplied by: softmax scale times 2^(E - up), in two steps (either may be far from 1)
-                        const int e = sm_E[tj & 3] - up_row;
+                        const int e = tile.E - up_row;
                         const float f = fminf(fmaxf(a.c * exp2i(e >> 1) * exp2i(e - (e >> 1)), 1e-37f), 3e38f);
                         float m_s = m_ref * exp2i(-e >> 1) * exp2i(-e - (-e >> 1));  // the reference in S's units
 #pragma unroll 1
@@ -381,26 +628,35 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                                 for (int i = 0; i < 32; i += 2)
                                     mx[i / 2 & 3] = max3(mx[i / 2 & 3], __uint_as_float(r[ch][i]), __uint_as_float(r[ch][i + 1]));
                             const float top = fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]));
-                            // ---- a new reference, where the maximum has outgrown the last by 2^8; a new R
+                            // ---- a new reference, where the maximum has outgrown the last by 2^8; a new R, where a row that
+                            // sees keys with it would leave f16's range or lose them there
                             const bool grew = f * (top - m_s) > 8.f;  // (from -infinity: any)
-                            if (__any_sync(0xffffffffu, grew) || raise) {
+                            const bool move = far_R && top > -INFINITY;
+                            if (__any_sync(0xffffffffu, grew || move)) {
                                 float fo = grew ? ex2(f * (m_s - top)) : 1.f;
                                 if (grew) {
                                     m_s = top;
                                     m_ref = top * exp2i(e >> 1) * exp2i(e - (e >> 1));
                                 }
                                 l *= fo;
-                                if (raise) {
-                                    if (j > 0) fo *= exp2i(max(R_ref - (R + 2), -126));
-                                    R_ref = R + 2;
-                                    raise = false;
-                                }
-                                if (j > 0 || h > 0) {
-                                    // Before the first half this row's O is complete up to tile j - 1 (S came after it);
-                                    // before the second, the first half's product may still be adding to it.
+                                if (!first || h > 0) {
+                                    // Before the first half this row's O is complete up to the turn before (S came after
+                                    // it); before the second, the first half's product may still be adding to it.
                                     if (h > 0) {
-                                        ok = warp_all_wait(bar(bars.h_full[x]), (tx + j) & 1, a.err, 72);
+                                        ok = warp_all_wait(bar(bars.h_full[x]), tx & 1, a.err, 72);
                                         tc_fence_after();
+                                    }
+                                    if (__any_sync(0xffffffffu, move)) {
+                                        // down only as far as what the row has summed stays within f32
+                                        const float most = most_of<D>(tm_o);
+                                        if (move) {
+                                            const int room = max(100 + 127 - (int)(__float_as_uint(most) >> 23), 0);
+                                            const int to = R > R_ref || most == 0.f ? R + 2 : max(R + 2, R_ref - room);
+                                            fo = R_ref - to < -126 ? 0.f : fo * exp2i(min(R_ref - to, 126));
+                                            R_ref = to;
+                                            far_R = false;
+                                            shift = min(max(7 + R - R_ref, -40), 7);
+                                        }
                                     }
 #pragma unroll 1
                                     for (int ch = 0; ch < D / 32; ch++) {
@@ -415,7 +671,6 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                             }
                             // ---- P = 2^((S - ref) f + shift), packed over S.  (The difference first: the rounding of ref f
                             // in the exponent of a fused S f - ref f outgrows f32 where scores pass 2^30.)
-                            const int shift = max(7 + R - R_ref, -100);  // at most 5
                             const float less = m_s == -INFINITY ? 0.f : -m_s, up = (float)shift;
                             const uint64_t less2 = pk2(less, less), f2 = pk2(f, f), up2 = pk2(up, up);
                             uint64_t sum2[2] = {0, 0};
@@ -435,7 +690,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                             }
                             float s0, s1;
                             upk2(add2(sum2[0], sum2[1]), s0, s1);
-                            l = fmaf(s0 + s1, exp2i(-shift), l);
+                            if (!tile.again) l = fmaf(s0 + s1, exp2i(-shift), l);
                             tmem_wait_st();
                             if (h == 0) hand_over(0);
                         }
@@ -449,6 +704,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         hand_over(1);
                     else
                         sm_gave_up = 1;  // (this warp goes on to the next barrier with the others)
+                    t++;
+                    tx++;
+                    first = false;
+                    last = j;
+                    if (!tile.more) j++;
                 }
                 // ---- the rows' outputs
                 if (all_ok) {
@@ -459,12 +719,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     sm_gave_up = 1;
                 }
                 if (ok && all_ok) {
-                    see_bad(n - 1);
+                    see_bad(last);
                     tc_fence_after();
                     const bool whole = p.unit0 == 0 && p.unit1 == p.kr.units;
                     const long long part_row = (2ll * blockIdx.x + (p.unit0 ? 0 : 1)) * PR_ROWS + x * 128 + row;
                     const int h = p.at.head * a.group + min(nr, rows - 1) - tok * a.group;
-                    const float back = exp2i(R_ref - 7), inv = l == 0.f ? 0.f : 1.f / l;
+                    // O 2^(R_ref - 7) / l, the power of two in two steps (it may be beyond f32's)
+                    const float back0 = (l == 0.f ? 0.f : 1.f / l) * exp2i((R_ref - 7) >> 1), back1 = exp2i(R_ref - 7 - ((R_ref - 7) >> 1));
                     // Through shared memory (the warp's part of Q, which nothing reads any more), so that a store
                     // covers whole rows of 128 bytes: 64 channels in bf16, 32 in f32.
                     const uint32_t stage = base + C::Q_OFF + x * C::Q + (warp & 3) * 4096;
@@ -476,8 +737,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         const bool nan = poison >> (32 * ch / KV4_GROUP) & 1;
 #pragma unroll
                         for (int i = 0; i < 32; i++) {
-                            const float v = nan ? NAN : l == 0.f ? 0.f : __uint_as_float(r[i]) * back;
-                            r[i] = __float_as_uint(whole ? v * inv : v);
+                            r[i] = __float_as_uint(nan ? NAN : l == 0.f ? 0.f : __uint_as_float(r[i]) * back0 * back1);
                         }
                         const float* f = (const float*)r;
                         if (whole) {
@@ -517,16 +777,18 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     }
                     tc_fence_before();
                 }
-                tx += n;
                 rounds++;
             }
-            t += n;
             // (nobody leaves before all eight warps are here)
             if (!ok) sm_gave_up = 1;
             named_bar(1, PR_SOFTMAX * 32);
-            if (warp == 0) sm_go[3][0] = !sm_gave_up;
+            if (warp == 0) {
+                sm_go[3][0] = !sm_gave_up;
+                sm_t = t;
+            }
             named_bar(1, PR_SOFTMAX * 32);
             ok = sm_go[3][0];
+            t = sm_t;  // (B may have had no rows)
             if (!ok) break;
             if (p.unit0 != 0 || p.unit1 != p.kr.units) {
                 // ---- a piece of a split tile: the last to finish joins them
@@ -534,7 +796,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 if (tid == 0) sm_last = last_piece(a, c0, c1);
                 named_bar(1, PR_SOFTMAX * 32);
                 if (sm_last)
-                    join_tile<D, PR_ROWS, PR_SOFTMAX * 32, 512>(a, s, p.at.head, n0, min(PR_ROWS, rows - n0), c0, c1, sm,
+                    join_tile<D, PR_ROWS, PR_SOFTMAX * 32, 512, true>(a, s, p.at.head, n0, min(PR_ROWS, rows - n0), c0, c1, sm,
                                                                 sm_join);
             }
             if (!pieces[(turn + 1) % RING].any) break;
@@ -549,7 +811,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
         const int kk = (w & 3) * 32 + lane, kh = w >> 2, vk = (w & 3) * 4 + (lane & 3), vc = (w >> 2) * 8 + (lane >> 2);
         const bool v_on = vc < D / 8;
         const int vg = 8 * vc / KV4_GROUP;
-        uint32_t t = 0, events = 0;
+        uint32_t t = 0, events = 0, marks = 0;  // (marks: K's stages that hold such, a bit each)
         for (int turn = 0; ok; turn++) {
             const Piece& p = pieces[turn % RING];
             if (w == 0 && lane == 0) next_piece<PR_ROWS, PR_KEYS>(a, sh, p, pieces[(turn + 1) % RING]);
@@ -611,7 +873,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             auto load_values = [&](const uint8_t* kb, const uint8_t* vb) {
                 const uint4* src = (const uint4*)(kb + kat * (D / 2) + kh * (D / 4));
 #pragma unroll
-                for (int i = 0; i < KW / 4; i++) *(uint4*)(kw + 4 * i) = __ldg(src + i);
+                for (int i = 0; i < KW / 4; i++) {
+                    const uint4 y = __ldg(src + i);
+                    kw[4 * i] = y.x; kw[4 * i + 1] = y.y; kw[4 * i + 2] = y.z; kw[4 * i + 3] = y.w;
+                }
                 if (v_on) {
                     const uint32_t* src = (const uint32_t*)(vb + half + vat * (D / 2)) + vc;
 #pragma unroll
@@ -631,127 +896,77 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
             kid = k_id(2);
             vid = v_id(2);
             for (int j = 0; j < n; j++) {
-                const uint32_t tj = t + j, st = tj & 1;
-                // ---- the tile's powers of two, from the bf16 bits of all scales and zeros
-                if (keep != 0x1ffu) {
+                const uint32_t tj = t, st = tj & 1;
+                // ---- whether its scales and zeros fit E and R
+                const uint4 fit = sm_far.fit;
+                if (keep != 0x1ffu) {  // keys that are not wanted: the smallest that fits
 #pragma unroll
-                    for (int i = 0; i < NG; i++) kp[i] = keep & 256u ? kp[i] : 0u;
+                    for (int i = 0; i < NG; i++) kp[i] = keep & 256u ? kp[i] : (0u - fit.x) & 0xffffu;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) vp[i] = keep >> i & 1 ? vp[i] : 0u;
+                    for (int i = 0; i < 8; i++) vp[i] = keep >> i & 1 ? vp[i] : (0u - fit.z) & 0xffffu;
                 }
-                uint32_t kt = 0, vt = 0;
+                uint32_t kx = 0, vx = 0;
 #pragma unroll
-                for (int i = 0; i < NG; i++) kt = umax2(kt, kp[i] & 0x7fff7fffu);
+                for (int i = 0; i < NG; i++) kx = umax2(kx, uadd2(kp[i] & 0x7fff7fffu, fit.x));
 #pragma unroll
-                for (int i = 0; i < 8; i++) vt = umax2(vt, vp[i] & 0x7fff7fffu);
-                uint32_t bad = 0;
-                if ((kt & 0xffffu) >= 0x7f80u || kt >= 0x7f800000u) kt = 0;  // a NaN needs no power of two
-                if ((vt & 0xffffu) >= 0x7f80u || vt >= 0x7f800000u) {
-                    vt = 0;
-#pragma unroll
-                    for (int i = 0; i < 8; i++) {
-                        if ((vp[i] & 0x7f80u) == 0x7f80u || (vp[i] & 0x7f800000u) == 0x7f800000u) {
-                            bad |= 1u << i;
-                            vp[i] = 0;
-                        }
-                        vt = umax2(vt, vp[i] & 0x7fff7fffu);
-                    }
-                }
-#pragma unroll
-                for (int i = 16; i; i >>= 1) {
-                    kt = umax2(kt, __shfl_xor_sync(0xffffffffu, kt, i));
-                    vt = umax2(vt, __shfl_xor_sync(0xffffffffu, vt, i));
-                }
-                if (lane == 0) sm_top[st][w] = make_uint2(kt, vt);
+                for (int i = 0; i < 8; i++) vx = umax2(vx, uadd2(vp[i] & 0x7fff7fffu, fit.z));
+                const bool odd = umax2(kx, fit.y) != fit.y || (v_on && umax2(vx, fit.w) != fit.w) || (marks >> st & 1);
                 // one warp waits for K's stage, the others for it
                 if (w == 0)
                     sm_go[2][events & 1] =
                         (tj < 2 || warp_all_wait(bar(bars.k_empty[st]), ((tj >> 1) - 1) & 1, a.err, 63)) && !sm_gave_up;
-                named_bar(2, PR_UNPACK * 32);
+                const bool far = named_bar_any(2, PR_UNPACK * 32, odd);
                 ok = sm_go[2][events++ & 1];
                 if (!ok) break;
+                bool done = false;
+                if (far) {
+                    if (kh == 0) {
 #pragma unroll
-                for (int i = 0; i < PR_UNPACK; i++) {
-                    kt = umax2(kt, sm_top[st][i].x);
-                    vt = umax2(vt, sm_top[st][i].y);
-                }
-                // K: scales below 2^-8, c below 2^6; V: scales below 2^-8, zeros below 2^13
-                const int E = min(max(max(bexpo(kt) + 9, bexpo(kt >> 16) - 4), -100), 120);
-                const int R = min(max(max(bexpo(vt) + 9, bexpo(vt >> 16) - 12), -100), 110);
-                // ---- K
-                {
-                    const float sc = __uint_as_float((kh == 0 ? kp[0] : kp[NG - 1]) << 16);
-                    const float s24 = sc * exp2i(24 - E), m8 = -8.f * (sc * exp2i(-E));
-                    const uint32_t sl = half2_bits(s24, s24), sh_ = half2_bits(s24 * 0x1p-4f, s24 * 0x1p-4f),
-                                   off = half2_bits(m8, m8);
-                    const uint32_t dst = base + C::K_OFF + st * C::K + (NG == 2 ? kh * C::ATOM : 0) + kk * 128 + ((kk & 7) << 4);
-#pragma unroll
-                    for (int i = 0; i < KW; i++) {
-                        const uint32_t lo = kw[i], hi = lo >> 8;
-                        const int chunk = NG == 2 ? i : kh * KW + i;
-                        sts128(dst ^ (chunk << 4), hfma2(lo & 0x000f000fu, sl, off), hfma2(lo & 0x00f000f0u, sh_, off),
-                               hfma2(hi & 0x000f000fu, sl, off), hfma2(hi & 0x00f000f0u, sh_, off));
+                        for (int i = 0; i < NG; i++) sm_far.kp[i][kk] = keep & 256u ? kp[i] : 0u;
                     }
-                }
-                if (kh == 0) {
-                    // (hi, hi, lo, lo) of each group, against the row's (hi, lo, hi, lo)
-                    uint32_t cw[2] = {0, 0};
+                    if (v_on && (vc & 7) == 0) {
 #pragma unroll
-                    for (int gr = 0; gr < NG; gr++)
-                        cw[gr] = split_half(fmaf(8.f, __uint_as_float(kp[gr] << 16), __uint_as_float(kp[gr] & 0xffff0000u)) *
-                                            exp2i(-E) * 256.f);
-                    sts128(base + C::KX_OFF + st * C::X + kk * 32 + ((kk >> 2 & 1) << 4), __byte_perm(cw[0], 0, 0x1010),
-                           __byte_perm(cw[0], 0, 0x3232), __byte_perm(cw[1], 0, 0x1010), __byte_perm(cw[1], 0, 0x3232));
+                        for (int i = 0; i < 8; i++) sm_far.vp[vg][8 * vk + i] = keep >> i & 1 ? vp[i] : 0u;
+                    }
                     if (w == 0 && lane == 0) {
-                        sm_E[tj & 3] = E;
-                        sm_R[tj & 3] = R;
+                        sm_far.tile0 = k0 + j * PR_KEYS;
+                        sm_far.end = k1;
+                        sm_far.t = t;
+                        sm_far.piece = turn % RING;
                     }
+                    named_bar(3, PR_UNPACK * 32 + 32);
+                    named_bar(3, PR_UNPACK * 32 + 32);
+                    done = sm_far.done;
+                    t = sm_far.t;
+                    marks = sm_far.marks;
+                    if (!(ok = sm_far.ok)) break;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) {
-                    mbar_arrive(bar(bars.k_full[st]));
-                    mbar_arrive(bar(bars.f_full[tj & 3]));
-                }
-                // ---- V
-                if (tj >= 2) {
-                    if (w == 0)
-                        sm_go[2][events & 1] = warp_all_wait(bar(bars.v_empty[st]), ((tj >> 1) - 1) & 1, a.err, 65) && !sm_gave_up;
-                    named_bar(2, PR_UNPACK * 32);
-                    ok = sm_go[2][events++ & 1];
-                    if (!ok) break;
-                }
-                if (v_on) {
-                    const float up = exp2i(24 - R), down = exp2i(-R);
-                    uint32_t sl[4], sh_[4], ze[4];  // of two keys: scale * 2^24 and 2^20, zero, times 2^-R
-#pragma unroll
-                    for (int i = 0; i < 4; i++) {
-                        const uint32_t p0 = vp[2 * i], p1 = vp[2 * i + 1];
-                        const float s0 = __uint_as_float(p0 << 16) * up, s1 = __uint_as_float(p1 << 16) * up;
-                        sl[i] = half2_bits(s0, s1);
-                        sh_[i] = half2_bits(s0 * 0x1p-4f, s1 * 0x1p-4f);
-                        ze[i] = half2_bits(__uint_as_float(p0 & 0xffff0000u) * down, __uint_as_float(p1 & 0xffff0000u) * down);
+                if (!done) {
+                    const int E = sm_far.E;
+                    // ---- K
+                    put_k<D>(base, st, kk, kh, kw, kp, E);
+                    if (w == 0 && lane == 0) *(int4*)&sm_tile[tj & 3] = make_int4(E, sm_far.R, 0, 0);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) {
+                        mbar_arrive(bar(bars.k_full[st]));
+                        mbar_arrive(bar(bars.f_full[tj & 3]));
                     }
-                    if ((vc & 7) == 0) sm[C::N_OFF + (tj & 3) * 32 + vg * 16 + vk] = (uint8_t)bad;
-                    const uint32_t dst = base + C::V_OFF + st * C::V + (vk >> 3) * (D * 128) + vc * 1024 + ((vk & 7) << 4);
-#pragma unroll
-                    for (int b = 0; b < 4; b++) {
-                        const uint32_t sel = b | (b << 4) | ((4 + b) << 8) | ((4 + b) << 12);
-                        uint32_t lo[4], hi[4];
-#pragma unroll
-                        for (int i = 0; i < 4; i++) {
-                            const uint32_t y = __byte_perm(vw[2 * i], vw[2 * i + 1], sel);
-                            lo[i] = hfma2(y & 0x000f000fu, sl[i], ze[i]);
-                            hi[i] = hfma2(y & 0x00f000f0u, sh_[i], ze[i]);
-                        }
-                        const int r0 = 2 * b, r1 = 2 * b + 1;  // channels 8 vc + r
-                        sts128((dst ^ (r0 << 4)) + r0 * 128, lo[0], lo[1], lo[2], lo[3]);
-                        sts128((dst ^ (r1 << 4)) + r1 * 128, hi[0], hi[1], hi[2], hi[3]);
+                    // ---- V
+                    if (tj >= 2) {
+                        if (w == 0)
+                            sm_go[2][events & 1] =
+                                warp_all_wait(bar(bars.v_empty[st]), ((tj >> 1) - 1) & 1, a.err, 65) && !sm_gave_up;
+                        named_bar(2, PR_UNPACK * 32);
+                        ok = sm_go[2][events++ & 1];
+                        if (!ok) break;
                     }
+                    if (v_on) put_v<D>(base, sm, st, tj, vk, vc, vw, vp, sm_far.R);
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
+                    t++;
                 }
-                fence_proxy_async_smem();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(bars.v_full[st]));
                 // Everything that an earlier load brought is taken first, then all new loads are issued together (a
                 // load ahead of such a use was waited for with it).
                 next_params();
@@ -762,13 +977,119 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 kid = k_id(j + 3);
                 vid = v_id(j + 3);
             }
-            t += n;
             // the next piece was made by this warpgroup's first thread, and its
             // tiles' barrier 2 has ordered that before
             if (!ok || !pieces[(turn + 1) % RING].any) break;
         }
+        if (w == 0 && lane == 0) sm_far.piece = -1;
+        named_bar(3, PR_UNPACK * 32 + 32);  // (the helper leaves)
     } else {
         regs_down<PR_REGS_MMA>();
+        if (warp == PR_HELP_WARP) {
+            // ======== tiles whose keys' magnitudes are too far apart, in as
+            // many turns as they need.  The unpacking warps wait meanwhile: what
+            // such a tile takes stays out of their loop, whose registers are
+            // full.  (Rare, so written for few instructions.)
+            uint32_t marks = 0;
+            for (;;) {
+                named_bar(3, PR_UNPACK * 32 + 32);
+                if (sm_far.piece < 0) break;
+                const Piece& p = pieces[sm_far.piece];
+                const int P = a.pool.page_tokens, half = P * (D / 2), tile0 = sm_far.tile0, end = sm_far.end;
+                uint32_t t = sm_far.t;
+                bool done = false;
+                auto words = [&](int key, int v) -> const uint32_t* {  // a key's values, nullptr where it is not wanted
+                    if (key < p.kr.first || key >= end) return nullptr;
+                    const int id = a.pages[(long long)p.at.b * a.max_pages + (key >> a.pool.page_shift)];
+                    if (id < 0 || id >= a.pool.pages) return nullptr;
+                    return (const uint32_t*)(a.pool.data + (long long)p.at.head * a.pool.block + (long long)id * a.pool.page_stride +
+                                             v * half + (key & (P - 1)) * (D / 2));
+                };
+                for (int pass = 0;; pass++) {
+                    const uint32_t st = t & 1;
+                    if (pass && !(ok = warp_all_wait(bar(bars.k_empty[st]), ((t >> 1) - 1) & 1, a.err, 74) && !sm_gave_up)) break;
+                    const bool apart = pick_keys(sm_tile[t & 3], sm_far, NG, pass);
+                    __syncwarp();
+                    const PromptTile tile = sm_tile[t & 3];
+                    if (pass == 0) {
+                        done = apart || (marks >> st & 1);
+                        if (!done) {  // the unpacking warps go on with these
+                            if (lane == 0) {
+                                const uint2 k = fitting(tile.E - 9, tile.E - 9 - K_WIDE, tile.E + 4),
+                                            v = fitting(tile.R - 9, tile.R - 9 - V_WIDE, tile.R + 12);
+                                sm_far.fit = make_uint4(k.x, k.y, v.x, v.y);
+                                sm_far.E = tile.E;
+                                sm_far.R = tile.R;
+                                sm_far.set = true;
+                            }
+                            break;
+                        }
+                    }
+                    marks &= ~(1u << st);
+#pragma unroll 1
+                    for (int kk = lane; kk < PR_KEYS; kk += 32) {
+                        const bool on = sm_far.keys[kk >> 5] >> lane & 1;
+                        const uint32_t* src = on ? words(tile0 + kk, 0) : nullptr;
+                        uint32_t cw[2] = {0, 0};
+#pragma unroll
+                        for (int gr = 0; gr < NG; gr++) {
+                            const uint32_t kp = on ? sm_far.kp[gr][kk] : 0u;
+                            const K4 k(kp, tile.E);
+                            cw[gr] = K4::extra(kp, tile.E);
+                            const uint32_t dst = base + C::K_OFF + st * C::K + gr * C::ATOM + kk * 128 + ((kk & 7) << 4);
+#pragma unroll 1
+                            for (int i = 0; i < 8; i++) k.put(dst ^ (i << 4), src ? src[8 * gr + i] : 0u);
+                        }
+                        put_extra<D>(base, st, kk, cw);
+                        // 1 of every row times -infinity
+                        sts128(base + C::KX_OFF + st * C::X + kk * 32 + ((1 ^ (kk >> 2 & 1)) << 4), on ? 0u : 0xfc00u, 0, 0, 0);
+                        if (__any_sync(0xffffffffu, !on)) marks |= 1u << st;
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane < PR_UNPACK) {
+                        mbar_arrive(bar(bars.k_full[st]));
+                        mbar_arrive(bar(bars.f_full[t & 3]));
+                    }
+                    if (t >= 2 && !(ok = warp_all_wait(bar(bars.v_empty[st]), ((t >> 1) - 1) & 1, a.err, 75) && !sm_gave_up)) break;
+#pragma unroll 1
+                    for (int kk = lane; kk < PR_KEYS; kk += 32) {
+                        const bool on = sm_far.keys[kk >> 5] >> lane & 1;
+                        const uint32_t* src = on ? words(tile0 + kk, 1) : nullptr;
+                        const uint32_t dst = base + C::V_OFF + st * C::V + (kk >> 6) * (D * 128) + (kk & 7) * 2;
+#pragma unroll 1
+                        for (int gr = 0; gr < NG; gr++) {
+                            uint32_t vp = src && (sm_far.values[gr][kk >> 5] >> lane & 1) ? sm_far.vp[gr][kk] : 0u;
+                            const unsigned bad = __ballot_sync(0xffffffffu, !finite2(vp));
+                            if (!finite2(vp)) vp = 0;
+                            const float up = exp2i(24 - tile.R), s = __uint_as_float(vp << 16) * up,
+                                        z = __uint_as_float(vp & 0xffff0000u) * up * 0x1p-24f;
+                            const uint32_t sl = half2_bits(s, s), ze = half2_bits(z, z);
+#pragma unroll 1
+                            for (int i = 0; i < 64; i++) {  // (channel by channel, as the unpacking warps' words are)
+                                const uint32_t word = src ? src[8 * gr + (i >> 3)] : 0u;
+                                const uint32_t y = hfma2(word >> 4 * (i & 7) & 15u, sl, ze);
+                                sts16(dst + (64 * gr + i) * 128 + (((kk >> 3 & 7) ^ (i & 7)) << 4), y);
+                            }
+                            if ((lane & 7) == 0)
+                                sm[C::N_OFF + (t & 3) * 32 + gr * 16 + (kk >> 3)] = (uint8_t)(bad >> lane);
+                        }
+                    }
+                    fence_proxy_async_smem();
+                    __syncwarp();
+                    if (lane < PR_UNPACK) mbar_arrive(bar(bars.v_full[st]));
+                    t++;
+                    if (!tile.more) break;
+                }
+                if (lane == 0) {
+                    sm_far.t = t;
+                    sm_far.marks = marks;
+                    sm_far.done = done;
+                    sm_far.ok = ok;
+                }
+                named_bar(3, PR_UNPACK * 32 + 32);
+            }
+        }
         if (warp == PR_MMA_WARP) {
             // ======== the tensor core
             const uint32_t lead = elect_one();
@@ -805,8 +1126,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 qk(0, t & 1);
                 if (two) qk(1, t & 1);
                 commit_if(lead, bar(bars.k_empty[t & 1]));
-                for (int j = 0; j < n && ok; j++, t++) {
+                bool first = true, last = false;
+                for (int j = 0; ok && !last; t++) {
                     const uint32_t st = t & 1, nt = t + 1;
+                    const bool more = sm_tile[t & 3].more;  // (came with K)
+                    last = !more && j + 1 == n;
                     ok = wait(bars.v_full[st], t >> 1 & 1, 68);
 #pragma unroll
                     for (int x = 0; x < 2; x++) {
@@ -814,7 +1138,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         ok = ok && wait(bars.p_full[x][0], tx[x] & 1, 69);
                         if (!ok) break;
                         tc_fence_after();
-                        pv(x, st, 0, j == 0);
+                        pv(x, st, 0, first);
                         commit_if(lead, bar(bars.h_full[x]));
                         ok = wait(bars.p_full[x][1], tx[x] & 1, 73);
                         if (!ok) break;
@@ -822,7 +1146,7 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         tc_fence_after();
                         pv(x, st, 1, false);
                         if (x == (two ? 1 : 0)) commit_if(lead, bar(bars.v_empty[st]));
-                        if (j + 1 < n) {
+                        if (!last) {
                             if (x == 0) ok = wait(bars.k_full[nt & 1], nt >> 1 & 1, 67);
                             if (!ok) break;
                             tc_fence_after();
@@ -830,7 +1154,9 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         } else
                             commit_if(lead, bar(bars.o_full[x]));
                     }
-                    if (ok && j + 1 < n) commit_if(lead, bar(bars.k_empty[nt & 1]));
+                    if (ok && !last) commit_if(lead, bar(bars.k_empty[nt & 1]));
+                    first = false;
+                    if (!more) j++;
                 }
                 if (!ok || !pieces[(turn + 1) % RING].any) break;
             }

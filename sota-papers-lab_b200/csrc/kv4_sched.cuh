@@ -279,8 +279,8 @@ __device__ __forceinline__ bool last_piece(const Kv4Attend& a, int c0, int c1) {
 // Joins the pieces that CTAs c0 .. c1 left of a tile's `cols` columns from row
 // n0 on; THREADS threads call it and meet at named barrier 1.  D/4 threads hold a column's channels; where columns are few, the
 // pieces of one are shared out among several such teams, which meet in `sm`
-// (32 lanes' part every WARP bytes) and `sm_ml` [THREADS / (D/4)].
-template <int D, int COLS, int THREADS, int WARP>
+// (32 lanes' part every WARP bytes) and `sm_ml` [THREADS / (D/4)].  MEANS: the pieces' outputs are divided by their sums.
+template <int D, int COLS, int THREADS, int WARP, bool MEANS = false>
 __device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int head, int n0, int cols, int c0, int c1,
                                           uint8_t* sm, float2* sm_ml) {
     auto sync = [] { named_bar(1, THREADS); };
@@ -314,8 +314,9 @@ __device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int 
                 float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
                 for (int i = 0; i < 4; i++) {
-                    const float f = ex2(ml[k][i].x - ref);
+                    float f = ex2(ml[k][i].x - ref);
                     sum = fmaf(f, ml[k][i].y, sum);
+                    if (MEANS) f *= ml[k][i].y;
                     v.x = fmaf(f, y[k][i].x, v.x); v.y = fmaf(f, y[k][i].y, v.y);
                     v.z = fmaf(f, y[k][i].z, v.z); v.w = fmaf(f, y[k][i].w, v.w);
                 }
@@ -357,8 +358,9 @@ __device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int 
             v.x *= f0; v.y *= f0; v.z *= f0; v.w *= f0;
 #pragma unroll
             for (int i = 0; i < AHEAD; i++) {
-                const float f = ex2(ml[i].x - ref);
+                float f = ex2(ml[i].x - ref);
                 sum = fmaf(f, ml[i].y, sum);
+                if (MEANS) f *= ml[i].y;
                 v.x = fmaf(f, y[i].x, v.x); v.y = fmaf(f, y[i].y, v.y);
                 v.z = fmaf(f, y[i].z, v.z); v.w = fmaf(f, y[i].w, v.w);
             }

@@ -1135,3 +1135,92 @@ def huge_values(engines, d, size, rows):
 @pytest.mark.parametrize("rows", [3, 5, 40])
 def test_attend_huge_finite_values_stay_with_the_rows_that_see_them(engines, d, size, rows):
     huge_values(engines, d, size, rows)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e4, 1e8, 1e20, 1e30, 1e32, 2e37])
+def test_attend_prompt_huge_finite_values_stay_with_the_rows_that_see_them(engines, d, size):
+    huge_values(engines, d, size, 90)
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1e3, 1e6, 1e12, 1e30, 1e35])
+@pytest.mark.parametrize("rows", [5, 40, 90])
+def test_attend_huge_finite_keys_stay_with_the_rows_that_see_them(engines, d, size, rows):
+    """The same of a cached K: rows that do not see it score their other keys as if it were not there."""
+    n = 500
+    b = Batch(d, 16, 4, 2, [n], [rows], seed=rows, tail_rows=0)
+    hidden = n - rows + rows // 2
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    right, lse = b.out.clone(), b.lse.clone()
+    b.k[hidden] *= size
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    before = torch.arange(rows, device=DEV) < rows // 2
+    # the same scores up to f32's rounding: a step of bf16 at most, lse by a few of f32's steps of the scores
+    assert ((b.out - right).abs()[before] <= 2.0 ** -7 * right.abs()[before] + 1e-3).all()
+    assert ((b.lse - lse).abs()[before] <= 1e-4).all()
+    assert torch.isfinite(b.out[~before]).all()
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 3, 30, 90, 170])
+@pytest.mark.parametrize("window", [0, 100])
+def test_attend_of_any_magnitudes(engines, d, rows, window):
+    """Every key's K and V, and every query, with a power of two of its own: each key counts as much as it weighs."""
+    b = Batch(d, 32, 4, 2, [900, 333, 1500], [rows, min(rows, 64), rows], seed=rows + d, tail_rows=0)
+    g = gen(rows)
+
+    def scaled(x, low, high):
+        e = torch.rand(x.shape[:2], generator=g, device=DEV)[..., None] * (high - low) + low
+        return (x.float() * torch.exp2(e.round())).bfloat16()
+
+    b.k, b.q = scaled(b.k, -30, 0), scaled(b.q, -20, 1)
+    b.v = scaled(b.v, -40, 60)
+    b.v[::7, 0] = 0.0
+    b.k[3::11, 1] = 0.0
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], window=window)
+    check_attend(b, "magnitudes", window=window)
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [4, 90])
+def test_attend_far_keys_on_a_long_cache(engines, d, rows):
+    """The same where tiles are cut and joined: a few huge and a few tiny keys among 9000, one V that is not finite and
+    that half the queries see."""
+    n = 9000
+    b = Batch(d, 64, 4, 1, [n], [rows], seed=rows + d, tail_rows=0)
+    b.v[::501] *= 2.0 ** 70
+    b.v[100::333] *= 2.0 ** -50
+    b.k[50::777] *= 2.0 ** -40
+    b.v[n - rows + rows // 2, 0, 3] = math.inf
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    first = b.out.clone()
+    b.attend(engines[d], engines["ws", d])
+    half = rows // 2
+    assert torch.equal(b.out[:half], first[:half]) and torch.isnan(b.out[half:, :, :64]).all()
+    b.v[n - rows + half, 0, 3] = 1.0  # (the rows that do not see it, and its other group, are right)
+    b.fill(engines[d])
+    for row, o, lse, size in exact_attend(b):
+        bad = (first.double() - o).abs() > 2.0 ** -8 * o.abs() + (2.0 ** -9 + 2.0 ** -15) * size
+        assert not bad[:half].any() and not bad[half:, :, 64:].any()
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("rows", [3, 40, 90])
+@pytest.mark.parametrize("size", [1e4, 1e9, 1e25])
+def test_attend_groups_of_v_far_apart(engines, rows, size):
+    """One half of V's channels far larger than the other, in all keys or in some: the other keeps its precision."""
+    b = Batch(128, 32, 4, 2, [700, 90], [rows, 1], seed=rows, tail_rows=0)
+    b.v[:, 0, 64:] *= size
+    b.v[::3, 1, :64] *= size
+    b.v[1::5, 1, 64:] /= size
+    b.fill(engines[128])
+    b.attend(engines[128], engines["ws", 128])
+    check_attend(b, "groups")
+    engines[128].engine_status()
