@@ -22,7 +22,7 @@
 //   - V's n enters the same way.  Its scale goes into the probability, in f16:
 //     p * s * 2^(14 - R) is rounded once by 2^-11 of itself (2^-25 * 2^-14 of
 //     2^R where it is subnormal).  R follows the magnitudes of the scales that
-//     the warp meets, within [2^(R - 16), 2^(R + 1)]; the few keys of a step
+//     the warp meets, within [2^(R - 12), 2^(R + 1)]; the few keys of a step
 //     whose scale lies outside while others' do not are added to the sums in
 //     f32, one by one, so that no key takes precision from the rows that do
 //     not see it.  sum(p z) is kept in f32.
@@ -182,19 +182,19 @@ __device__ __forceinline__ void load_step(const Kv4Attend& a, uint32_t stage, co
     }
 }
 
-// V's scales in f16: R with 2^(R - 16) <= |s| < 2^(R + 1) for those that are held (as bf16 bits less `low`, at
+// V's scales in f16: R with 2^(R - 12) <= |s| < 2^(R + 1) for those that are held (as bf16 bits less `low`, at
 // most V_SPAN; bits of another sign or of NaN are not).
-constexpr uint32_t V_SPAN = (17u << 7) * 0x10001u, V_UNSET = 0x80008000u;
+constexpr uint32_t V_SPAN = (13u << 7) * 0x10001u, V_UNSET = 0x80008000u;
 // |s|, 0 where it is not finite (such a key comes out as NaN in the rows that see it whatever R is).
 __device__ __forceinline__ float scale_size(float s) { return fabsf(s) < INFINITY ? fabsf(s) : 0.f; }
 __device__ __forceinline__ int scale_R(float top) { return max((int)(__float_as_uint(top) >> 23) - 126, -100); }  // top < 2^R
 __device__ __forceinline__ int up_R(float v_up) { return 14 + 127 - (int)(__float_as_uint(v_up) >> 23); }         // 2^(14 - R)
 __device__ __forceinline__ bool scale_fits(float size, int R) {
-    return size == 0.f || (size >= exp2i(R - 16) && size <= exp2i(min(R + 1, 127)));
+    return size == 0.f || (size >= exp2i(R - 12) && size <= exp2i(min(R + 1, 127)));
 }
 template <int NG>
 __device__ __forceinline__ void set_low(uint32_t& v_low, int gr, int R) {
-    const uint32_t low = 0x10000u - (uint32_t)((R - 16 + 127) << 7), in_gr = NG == 1 ? 0xffffffffu : 0xffffu << 16 * gr;
+    const uint32_t low = 0x10000u - (uint32_t)((R - 12 + 127) << 7), in_gr = NG == 1 ? 0xffffffffu : 0xffffu << 16 * gr;
     v_low = (v_low & ~in_gr) | (low * 0x10001u & in_gr);
 }
 
