@@ -136,6 +136,22 @@ __device__ __forceinline__ void sts128(uint32_t p, uint32_t a, uint32_t b, uint3
 __device__ __forceinline__ void sts16(uint32_t p, uint32_t v) {
     asm volatile("st.shared.b16 [%0], %1;" ::"r"(p), "h"((uint16_t)v) : "memory");
 }
+// Plain loads, not read-only ones (ld.global.nc): the kernel may start while
+// the append before it still writes the pool.  As statements that depend on
+// their address alone, they can be moved between others as those can be (as C++
+// loads they stay behind every barrier: 611 us instead of 583); none can come
+// before griddep_wait, since all addresses follow from what is read after it.
+__device__ __forceinline__ uint32_t ld_pool(const uint32_t* p) {
+    uint32_t v;
+    asm("ld.global.u32 %0, [%1];" : "=r"(v) : "l"(p));
+    return v;
+}
+__device__ __forceinline__ int ld_pool(const int* p) { return (int)ld_pool((const uint32_t*)p); }
+__device__ __forceinline__ uint4 ld_pool(const uint4* p) {
+    uint4 v;
+    asm("ld.global.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+    return v;
+}
 template <int N>
 __device__ __forceinline__ void regs_up() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
 template <int N>
@@ -831,8 +847,8 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 const int key = vkey + j * PR_KEYS, lo = max(first - key, 0), hi = min(k1 - key, 8);
                 return j < n && v_on && lo < hi ? (0xffu >> (8 - hi)) & (0xffu << lo) : 0u;
             };
-            auto k_id = [&](int j) { return k_on(j) ? __ldg(ids + ((kkey + j * PR_KEYS) >> a.pool.page_shift)) : 0; };
-            auto v_id = [&](int j) { return v_mask(j) ? __ldg(ids + ((vkey + j * PR_KEYS) >> a.pool.page_shift)) : 0; };
+            auto k_id = [&](int j) { return k_on(j) ? ld_pool(ids + ((kkey + j * PR_KEYS) >> a.pool.page_shift)) : 0; };
+            auto v_id = [&](int j) { return v_mask(j) ? ld_pool(ids + ((vkey + j * PR_KEYS) >> a.pool.page_shift)) : 0; };
             // A page's block of the head; page 0's (never used) where nothing is wanted or the id is bad.
             auto block_of = [&](int& id, bool wanted) {
                 const bool good = id >= 0 && id < a.pool.pages;
@@ -857,10 +873,10 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 const uint32_t* kpar = (const uint32_t*)(kb + 2 * half) + kat * NG;
                 const uint32_t* vpar = (const uint32_t*)(vb + 2 * half + P * NG * 4) + vat * NG + vg;
 #pragma unroll
-                for (int i = 0; i < NG; i++) kq[i] = __ldg(kpar + i);
+                for (int i = 0; i < NG; i++) kq[i] = ld_pool(kpar + i);
                 if (v_on) {
 #pragma unroll
-                    for (int i = 0; i < 8; i++) vq[i] = __ldg(vpar + i * NG);
+                    for (int i = 0; i < 8; i++) vq[i] = ld_pool(vpar + i * NG);
                 }
             };
             auto next_params = [&] {
@@ -874,13 +890,13 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                 const uint4* src = (const uint4*)(kb + kat * (D / 2) + kh * (D / 4));
 #pragma unroll
                 for (int i = 0; i < KW / 4; i++) {
-                    const uint4 y = __ldg(src + i);
+                    const uint4 y = ld_pool(src + i);
                     kw[4 * i] = y.x; kw[4 * i + 1] = y.y; kw[4 * i + 2] = y.z; kw[4 * i + 3] = y.w;
                 }
                 if (v_on) {
                     const uint32_t* src = (const uint32_t*)(vb + half + vat * (D / 2)) + vc;
 #pragma unroll
-                    for (int i = 0; i < 8; i++) vw[i] = __ldg(src + i * (D / 8));
+                    for (int i = 0; i < 8; i++) vw[i] = ld_pool(src + i * (D / 8));
                 }
             };
             kid = k_id(0);

@@ -1224,3 +1224,34 @@ def test_attend_groups_of_v_far_apart(engines, rows, size):
     b.attend(engines[128], engines["ws", 128])
     check_attend(b, "groups")
     engines[128].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+def test_appends_between_prompt_calls_without_a_pause(engines, d):
+    """Attend, append into the page that the last call read half filled, attend again, nothing else on the stream in
+    between: each call sees what was appended before it, as calls with a pause between them do."""
+    eng, ws, page, n = engines[d], engines["ws", d], 64, 150
+    b = Batch(d, page, 4, 2, [700], [n], seed=d, tail_rows=0)
+    cache = sage.Kv4Cache(b.pool, page, d)
+    steps = [range(i, i + 10) for i in range(n, 700, 10)]
+    lens = [ints([s[-1] + 1]) for s in steps]
+    outs = [torch.zeros(n, 4, d, dtype=torch.bfloat16, device=DEV) for _ in range(2 * len(steps))]
+
+    def run(outs, pause):
+        b.pool.zero_()
+        eng.kv4_append(cache, b.k[:n], b.v[:n], b.slots[:n])
+        torch.cuda.synchronize()
+        for s, kv, out in zip(steps, lens, outs):
+            sl = slice(s[0], s[-1] + 1)
+            eng.kv4_append(cache, b.k[sl], b.v[sl], b.slots[sl])
+            if pause:
+                torch.cuda.synchronize()
+            eng.kv4_attend(ws, cache, b.q, out, b.pages, kv, q_start=b.q_start, max_q=n)
+            if pause:
+                torch.cuda.synchronize()
+
+    run(outs[:len(steps)], True)
+    for _ in range(5):
+        run(outs[len(steps):], False)
+        assert all(torch.equal(x, y) for x, y in zip(outs, outs[len(steps):]))
+    eng.engine_status()
