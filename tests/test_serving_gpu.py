@@ -1255,3 +1255,19 @@ def test_appends_between_prompt_calls_without_a_pause(engines, d):
         run(outs[len(steps):], False)
         assert all(torch.equal(x, y) for x, y in zip(outs, outs[len(steps):]))
     eng.engine_status()
+
+
+@pytest.mark.parametrize("d,kv,rows,window", [(128, 16000, 40, 0), (64, 9000, 33, 0), (128, 20000, 75, 12000),
+                                              (64, 12000, 65, 7001), (128, 8200, 65, 0)])
+def test_attend_prompt_tiles_of_many_pieces(engines, d, kv, rows, window):
+    """A piece of a prompt on a long cache: its tiles (the last of 160, 132, 44, 4 and 4 rows) are cut into more than
+    four pieces each, joined the same way every time."""
+    b = Batch(d, 64, 4, 1, [kv], [rows], seed=kv, tail_rows=1)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], window=window)
+    b.check(window=window)
+    first, lse = b.out.clone(), b.lse.clone()
+    for _ in range(3):
+        b.attend(engines[d], engines["ws", d], window=window)
+        assert torch.equal(b.out, first) and torch.equal(b.lse, lse)
+    engines[d].engine_status()
