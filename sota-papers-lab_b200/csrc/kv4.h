@@ -78,7 +78,8 @@ struct Kv4Attend {
 // behind counts that must be zero before the first call.
 constexpr size_t KV4_COUNTS = 8192;  // bytes
 size_t kv4_scratch_bytes(int d, int sms);
-cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t st);
+// On `sms` SMs; `alone`: the others stay free (no CTA shares an SM with another).
+cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, bool alone, cudaStream_t st);
 // The same for many query rows (kv4_prompt.cu).
 size_t kv4_prompt_scratch_bytes(int d, int sms);
 cudaError_t launch_kv4_prompt(int d, const Kv4Attend& a, int sms, cudaStream_t st);

@@ -377,7 +377,8 @@ int spl_sage_kv4_attend(spl_sage* s, spl_sage_kv4_ws* ws, const spl_sage_kv4* ca
     a.scratch = ws->mem;
     a.err = s->err;
     if ((rc = check_device(call, s))) return rc;
-    const cudaError_t e = sp::launch_kv4_attend(s->head_dim, a, s->sm_count - s->reserved_sms, s->stream);
+    const cudaError_t e = sp::launch_kv4_attend(s->head_dim, a, s->sm_count - s->reserved_sms,
+                                                s->reserved_sms > 0, s->stream);
     if (e != cudaSuccess) return cuda_fail(e, "launch the cache attention");
     return SPL_SAGE_OK;
 }

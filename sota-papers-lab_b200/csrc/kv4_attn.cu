@@ -826,14 +826,19 @@ size_t kv4_scratch_bytes(int d, int sms) {
 }
 
 template <int D, int NT>
-static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
+static cudaError_t attend(Kv4Attend a, int sms, bool alone, cudaStream_t st) {
     using C = AttnCfg<D, NT>;
     constexpr int COLS = C::COLS;
     // No more CTAs than the longest sequences that max_pages admits can give
     // work: those that have some get an SM to themselves then (one sequence of
     // 200, 1000, 3000 tokens: 6.3, 8.9, 9.3 us instead of 7.1, 10.0, 10.4).
     // The shares are the same.
-    const int full = (NT == 1 ? 2 : 1) * sms;
+    // With SMs reserved, no more CTAs than there are others, and with so much
+    // shared memory each that two cannot share an SM: CTAs are spread over idle
+    // SMs first, so that two for each of them would take the reserved ones as well.
+    constexpr int ALONE = std::max(C::SMEM, 116 * 1024);
+    const int smem = alone ? ALONE : C::SMEM;
+    const int full = (NT == 1 && !alone ? 2 : 1) * sms;
     const double tiles = (double)((a.max_q * a.group + COLS - 1) / COLS) * (a.heads / a.group) * a.batch;
     const long long units = (((long long)a.max_pages << a.pool.page_shift) + 31 + AT_UNIT - 1) / AT_UNIT;
     const int G = (int)std::min<double>(full, tiles * ((units + AT_LEAST - 1) / AT_LEAST));
@@ -846,14 +851,14 @@ static cudaError_t attend(Kv4Attend a, int sms, cudaStream_t st) {
     cudaError_t e = cudaGetDevice(&dev);
     if (e != cudaSuccess) return e;
     if (!(ready.load() >> (dev & 63) & 1)) {
-        e = cudaFuncSetAttribute(sp_kv4_attend<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, C::SMEM);
+        e = cudaFuncSetAttribute(sp_kv4_attend<D, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, ALONE);
         if (e != cudaSuccess) return e;
         ready.fetch_or(1ull << (dev & 63));
     }
-    return launch_after_previous(sp_kv4_attend<D, NT>, dim3(G), dim3(AT_WARPS * 32), C::SMEM, st, a);
+    return launch_after_previous(sp_kv4_attend<D, NT>, dim3(G), dim3(AT_WARPS * 32), smem, st, a);
 }
 
-cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t st) {
+cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, bool alone, cudaStream_t st) {
     const int rows = a.max_q * a.group;
     // Above 128 rows the tensor-core kernel with a tile of up to 256 rows, up
     // to there this one's tiles of 16 (which read the cache again from the L2).
@@ -861,8 +866,8 @@ cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, cudaStream_t s
     // rows 43 and 105, 64 rows 65 and 108, 128 rows 110 and 113, 256 rows 201
     // and 131; one sequence of 2000 tokens, 128 rows: 19 and 54.
     if (rows > 128) return launch_kv4_prompt(d, a, sms, st);
-    if (d == 64) return rows <= 8 ? attend<64, 1>(a, sms, st) : attend<64, 2>(a, sms, st);
-    return rows <= 8 ? attend<128, 1>(a, sms, st) : attend<128, 2>(a, sms, st);
+    if (d == 64) return rows <= 8 ? attend<64, 1>(a, sms, alone, st) : attend<64, 2>(a, sms, alone, st);
+    return rows <= 8 ? attend<128, 1>(a, sms, alone, st) : attend<128, 2>(a, sms, alone, st);
 }
 
 }  // namespace sp

@@ -1271,3 +1271,47 @@ def test_attend_prompt_tiles_of_many_pieces(engines, d, kv, rows, window):
         b.attend(engines[d], engines["ws", d], window=window)
         assert torch.equal(b.out, first) and torch.equal(b.lse, lse)
     engines[d].engine_status()
+
+
+def kernel_nodes(graph):
+    """(grid, dynamic shared memory) of a captured graph's kernels."""
+    from cuda.bindings import driver
+    err, _, n = driver.cuGraphGetNodes(graph.raw_cuda_graph(), 0)
+    assert int(err) == 0
+    err, nodes, n = driver.cuGraphGetNodes(graph.raw_cuda_graph(), n)
+    assert int(err) == 0
+    got = []
+    for x in nodes[:n]:
+        err, kind = driver.cuGraphNodeGetType(x)
+        if kind == driver.CUgraphNodeType.CU_GRAPH_NODE_TYPE_KERNEL:
+            err, p = driver.cuGraphKernelNodeGetParams(x)
+            assert int(err) == 0
+            got.append((p.gridDimX * p.gridDimY * p.gridDimZ, p.sharedMemBytes))
+    return got
+
+
+@pytest.mark.parametrize("reserved", [1, 20, 100])
+@pytest.mark.parametrize("d,rows", [(64, 1), (128, 1), (128, 4), (128, 60)])
+def test_attend_leaves_the_reserved_sms_free(d, rows, reserved):
+    """No more CTAs than SMs that are not reserved, and none of them able to share an SM with another call's (two
+    CTAs' shared memory is more than an SM has), so that they cannot be spread over more SMs than that either way."""
+    props = torch.cuda.get_device_properties(0)
+    s = torch.cuda.Stream()
+    with torch.cuda.stream(s):
+        eng = sage.SageAttention(s, d)
+        ws = eng.kv4_workspace()
+        b = Batch(d, 32, 8, 2, [9000, 900, 4000], [rows] * 3, seed=3)
+        b.fill(eng)
+        eng.reserve_sms(reserved)
+        b.attend(eng, ws)
+        s.synchronize()
+        b.check()
+        graph = torch.cuda.CUDAGraph(keep_graph=True)
+        with torch.cuda.graph(graph, stream=s):
+            b.attend(eng, ws)
+    grids = kernel_nodes(graph)
+    assert len(grids) == 1
+    grid, shared = grids[0]
+    assert grid <= props.multi_processor_count - reserved
+    assert 2 * shared > props.shared_memory_per_multiprocessor or rows == 60
+    del graph
