@@ -70,6 +70,36 @@ int64_t extent(int64_t st, int64_t sh, int64_t tokens, int64_t heads, int64_t d)
     return (tokens - 1) * st + (heads - 1) * sh + d;
 }
 
+// Whether a row of one [token][head][D] tensor overlaps a row of another (their
+// rows may lie between one another's: heads of one packed projection).  Element
+// sizes are the same.  Exact where the token strides are equal or one of them
+// is never used; otherwise by the range that each tensor spans.
+bool rows_meet(const void* a, int64_t ast, int64_t ash, int64_t ah, const void* b, int64_t bst, int64_t bsh, int64_t bh,
+               int64_t tokens, int64_t d, int64_t size) {
+    if (!ranges_meet(a, extent(ast, ash, tokens, ah, d) * size, b, extent(bst, bsh, tokens, bh, d) * size)) return false;
+    if (tokens > 1 && ast != bst) return true;
+    const int64_t off = (int64_t)((uintptr_t)b - (uintptr_t)a);  // in bytes
+    // rows i, j of a and k, l of b are off + (k - i) * st + l * bsh - j * ash apart
+    auto token_meets = [&](int64_t apart) {
+        if (tokens == 1 || ast == 0) return apart > -d * size && apart < d * size;
+        const int64_t st = ast * size, n = -(apart / st);  // the nearest token distances: n and one to either side
+        for (int64_t k = n - 1; k <= n + 1; k++)
+            if (k > -tokens && k < tokens && apart + k * st > -d * size && apart + k * st < d * size) return true;
+        return false;
+    };
+    if (ash == bsh || ah == 1 || bh == 1) {
+        const int64_t sh = (ah == 1 ? bsh : ash) * size;
+        for (int64_t m = 1 - ah; m < bh; m++)
+            if (token_meets(off + m * sh)) return true;
+        return false;
+    }
+    if (ah * bh > 1 << 16) return true;
+    for (int64_t j = 0; j < ah; j++)
+        for (int64_t l = 0; l < bh; l++)
+            if (token_meets(off + (l * bsh - j * ash) * size)) return true;
+    return false;
+}
+
 int check_rotary(const char* call, const spl_sage_rotary* r, const int32_t* positions, int head_dim,
                  sp::RotaryArgs* out) {
     *out = sp::RotaryArgs{};
@@ -242,10 +272,10 @@ int spl_sage_kv4_append(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, 
         if ((rc = check_rows("Q output", q_out.data, q_out.len, q_out.token, q_out.head, tokens, q_heads, d, true)))
             return rc;
         const bool in_place = q.data == q_out.data && q.token == q_out.token && q.head == q_out.head;
-        const int64_t n = extent(q_out.token, q_out.head, tokens, q_heads, d) * 2;
-        if (!in_place && (ranges_meet(q.data, extent(q.token, q.head, tokens, q_heads, d) * 2, q_out.data, n) ||
-                          ranges_meet(k.data, extent(k.token, k.head, tokens, hk, d) * 2, q_out.data, n) ||
-                          ranges_meet(v.data, extent(v.token, v.head, tokens, hk, d) * 2, q_out.data, n)))
+        auto meets = [&](const spl_sage_tensor& x, int64_t heads) {
+            return rows_meet(q_out.data, q_out.token, q_out.head, q_heads, x.data, x.token, x.head, heads, tokens, d, 2);
+        };
+        if ((!in_place && meets(q, q_heads)) || meets(k, hk) || meets(v, hk))
             return fail(SPL_SAGE_ERR_INVALID, "%s: the Q output overlaps an input without being Q", call);
     }
     if ((rc = check_device(call, s))) return rc;

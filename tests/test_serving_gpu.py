@@ -1315,3 +1315,31 @@ def test_attend_leaves_the_reserved_sms_free(d, rows, reserved):
     assert grid <= props.multi_processor_count - reserved
     assert 2 * shared > props.shared_memory_per_multiprocessor or rows == 60
     del graph
+
+
+@pytest.mark.parametrize("layout", ["rows", "heads", "per head", "one head"])
+def test_append_with_q_in_place(engines, layout):
+    """Q rotated where it lies, K and V beside it in the same buffer: token by token, head by head, q, k and v of a
+    head side by side, one head of each."""
+    d, eng, t, h, page = 128, engines[128], 70, 1 if layout == "one head" else 4, 16
+    g = gen(17)
+    if layout == "heads":
+        x = rand(g, 3 * h, t, d).transpose(0, 1)
+    else:
+        x = rand(g, t, 3 * h, d)
+    cut = [slice(0, h), slice(h, 2 * h), slice(2 * h, 3 * h)]
+    if layout == "per head":
+        cut = [slice(i, 3 * h, 3) for i in range(3)]
+    q, k, v = (x[:, c] for c in cut)
+    r, pos, slots = sage.Rotary(table(d, 100), d), ints(range(5, 5 + t)), ints(range(t))
+    pools = [torch.zeros(5, h, sage.Kv4Cache.block_bytes(d, page), dtype=torch.uint8, device=DEV) for _ in range(2)]
+    out = torch.empty(t, h, d, dtype=torch.bfloat16, device=DEV)
+    eng.kv4_append(sage.Kv4Cache(pools[0], page, d), k, v, slots, rotary=r, positions=pos, q=q, q_out=out)
+    keep = [k.clone(), v.clone()]
+    eng.kv4_append(sage.Kv4Cache(pools[1], page, d), k, v, slots, rotary=r, positions=pos, q=q, q_out=q)
+    assert torch.equal(*pools) and torch.equal(q, out) and torch.equal(k, keep[0]) and torch.equal(v, keep[1])
+    for other in (dict(k=q, v=v), dict(k=k, v=q), dict(k=x[:, 1:1 + h] if layout == "rows" else q, v=v)):
+        with pytest.raises(sage.SageError, match="overlaps an input"):
+            eng.kv4_append(sage.Kv4Cache(pools[1], page, d), other["k"], other["v"], slots, rotary=r, positions=pos, q=q,
+                           q_out=q)
+    eng.engine_status()

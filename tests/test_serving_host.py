@@ -237,3 +237,41 @@ def test_struct_layouts(sage, tmp_path):
     assert got == [ctypes.sizeof(sage._Rotary), ctypes.sizeof(sage._RopeScaling), ctypes.sizeof(sage._Kv4),
                    ctypes.sizeof(sage._Kv4Shape), sage._RopeScaling.attention.offset, sage._Kv4.kv_heads.offset,
                    sage._Kv4Shape.window.offset]
+
+
+@pytest.mark.parametrize("tokens", [1, 5])
+def test_append_q_output_over_k_or_v(calls, tokens):
+    """Q rotated in place beside K and V in one buffer is fine wherever the three lie; over a row of K or V it is not,
+    in place or not (every pair of rows is compared here)."""
+    c, d = calls, calls.d
+    c.mem[1:] = [(-1 << 32) | d] + [-1] * 14  # an engine of device -1: no call gets past the check of the device
+    base, hq, hk = 0x10000000, 4, 2
+
+    def rows(at, token, head, heads):
+        return [(at + 2 * (t * token + h * head), 2 * d) for t in range(tokens) for h in range(heads)]
+
+    layouts = []  # (token stride, head stride) of q, k, v and where k and v begin
+    packed = (hq + 2 * hk) * d
+    layouts.append(((packed, d), (packed, d), hq * d, (hq + hk) * d))            # token by token
+    layouts.append(((packed, d), (packed, d), (hq - 1) * d, (hq + hk) * d))      # k one head early: over q
+    layouts.append(((packed, d), (packed, d), hq * d, packed))                   # v over the next token's q
+    layouts.append(((d, tokens * d), (d, tokens * d), hq * tokens * d, (hq + hk) * tokens * d))  # head by head
+    layouts.append(((d, tokens * d), (d, tokens * d), (hq * tokens - 1) * d, (hq + hk) * tokens * d))
+    layouts.append(((packed, 2 * d), (packed, 4 * d), d, 3 * d))                 # between q's heads
+    layouts.append(((packed, 2 * d), (packed, 4 * d), d, 4 * d))
+    layouts.append(((packed, 2 * d), (packed, 4 * d), d + 64, 3 * d))            # half a row over
+    layouts.append(((packed, d), (packed, d), -64, (hq + hk) * d))
+    seen = set()
+    for (qs, ks, at_k, at_v) in layouts:
+        at = [base, base + 2 * at_k, base + 2 * at_v]
+        q = rows(at[0], *qs, hq)
+        apart = all(x + n <= y or y + m <= x for a, h in ((at[1], hk), (at[2], hk)) for x, n in rows(a, *ks, h) for y, m in q)
+        for q_in in (at[0], 0x70000000):  # in place, and from elsewhere
+            got = c.append(tokens=tokens, hq=hq, q=c.t(q_in, token=qs[0], head=qs[1]),
+                           q_out=c.t(at[0], token=qs[0], head=qs[1]), k=c.t(at[1], token=ks[0], head=ks[1]),
+                           v=c.t(at[2], token=ks[0], head=ks[1]))
+            # (what is fine gets as far as the device)
+            assert got != 0
+            assert (got != 0 and "overlaps an input" in c.why()) == (not apart), (qs, ks, at_k, at_v, c.why())
+        seen.add(apart)
+    assert seen == {True, False}
