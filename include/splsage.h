@@ -555,8 +555,9 @@ int spl_sage_kv4_append(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, 
                         int64_t q_heads, spl_sage_tensor q, spl_sage_tensor_mut q_out);
 
 /* The cached values at `slots`, zero + scale * n rounded to bf16, into k and v
- * [tokens][kv_heads][D] (e.g. a cached prefix for a dense kernel).  slots[t] <
- * 0: zeros; out of range: the rows are left as they were. */
+ * [tokens][kv_heads][D] (e.g. a cached prefix for a dense kernel), which must
+ * not overlap each other or the cache.  slots[t] < 0: zeros; out of range: the
+ * rows are left as they were. */
 int spl_sage_kv4_read(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, const int32_t* slots,
                       spl_sage_tensor_mut k, spl_sage_tensor_mut v);
 

@@ -299,6 +299,12 @@ int spl_sage_kv4_read(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, co
     const int64_t d = s->head_dim, hk = pool.kv_heads;
     if ((rc = check_rows("K", k.data, k.len, k.token, k.head, tokens, hk, d, true))) return rc;
     if ((rc = check_rows("V", v.data, v.len, v.token, v.head, tokens, hk, d, true))) return rc;
+    if (rows_meet(k.data, k.token, k.head, hk, v.data, v.token, v.head, hk, tokens, d, 2))
+        return fail(SPL_SAGE_ERR_INVALID, "%s: K and V overlap", call);
+    const int64_t pool_bytes = (pool.pages - 1) * pool.page_stride + (int64_t)pool.kv_heads * pool.block;
+    if (ranges_meet(k.data, extent(k.token, k.head, tokens, hk, d) * 2, pool.data, pool_bytes) ||
+        ranges_meet(v.data, extent(v.token, v.head, tokens, hk, d) * 2, pool.data, pool_bytes))
+        return fail(SPL_SAGE_ERR_INVALID, "%s: an output overlaps the cache", call);
     if ((rc = check_device(call, s))) return rc;
     const cudaError_t e = sp::launch_kv4_read(s->head_dim, pool, slots, {k.data, k.token, k.head},
                                               {v.data, v.token, v.head}, (int)tokens, s->err, s->stream);

@@ -275,3 +275,19 @@ def test_append_q_output_over_k_or_v(calls, tokens):
             assert (got != 0 and "overlaps an input" in c.why()) == (not apart), (qs, ks, at_k, at_v, c.why())
         seen.add(apart)
     assert seen == {True, False}
+
+
+def test_read_outputs_over_one_another(calls):
+    """K and V of a read may lie between one another's rows, but not on them, nor on the cache."""
+    c, d = calls, calls.d
+    c.mem[1:] = [(-1 << 32) | d] + [-1] * 14  # an engine of device -1: no call gets past the check of the device
+    at = 0x20000000
+    both = dict(token=4 * d, head=d)  # K and V heads of a token side by side
+    for k, v, text in ((c.t(at, heads=2), c.t(at, heads=2), "K and V overlap"),
+                       (c.t(at, **both), c.t(at + 2 * d, **both), "K and V overlap"),
+                       (c.t(at, token=2 * d, head=d), c.t(at + 2 * 9 * d, token=2 * d, head=d), "K and V overlap"),
+                       (c.t(0x900000000, heads=2), c.t(at, heads=2), "overlaps the cache"),
+                       (c.t(at, heads=2), c.t(0x900000000 + 9 * 18432, heads=2), "overlaps the cache")):
+        assert c.read(k=k, v=v) == 1 and text in c.why(), c.why()
+    assert c.read(k=c.t(at, **both), v=c.t(at + 4 * d, **both)) != 0 and "overlap" not in c.why()
+    assert c.read(k=c.t(at, token=2 * d, head=d), v=c.t(at + 2 * 10 * d, token=2 * d, head=d)) != 0 and "overlap" not in c.why()
