@@ -234,8 +234,7 @@ int spl_sage_rope(spl_sage* s, int dtype, int64_t tokens, int64_t heads, spl_sag
     if ((rc = check_rows("x", x.data, x.len, x.token, x.head, tokens, heads, d, false))) return rc;
     if ((rc = check_rows("output", out.data, out.len, out.token, out.head, tokens, heads, d, true))) return rc;
     const bool in_place = x.data == out.data && x.token == out.token && x.head == out.head;
-    if (!in_place && ranges_meet(x.data, extent(x.token, x.head, tokens, heads, d) * size, out.data,
-                                 extent(out.token, out.head, tokens, heads, d) * size))
+    if (!in_place && rows_meet(x.data, x.token, x.head, heads, out.data, out.token, out.head, heads, tokens, d, size))
         return fail(SPL_SAGE_ERR_INVALID, "%s: the output overlaps x without being x", call);
     if ((rc = check_device(call, s))) return rc;
     const cudaError_t e = sp::launch_rope(s->head_dim, dtype, {x.data, x.token, x.head}, {out.data, out.token, out.head},
@@ -381,8 +380,7 @@ int spl_sage_kv4_attend(spl_sage* s, spl_sage_kv4_ws* ws, const spl_sage_kv4* ca
     if ((uintptr_t)lse % 4) return fail(SPL_SAGE_ERR_INVALID, "%s: lse must start on 4 bytes", call);
     if ((rc = check_rows("Q", q.data, q.len, q.token, q.head, sh.tokens, sh.heads, d, false))) return rc;
     if ((rc = check_rows("output", out.data, out.len, out.token, out.head, sh.tokens, sh.heads, d, true))) return rc;
-    if (ranges_meet(q.data, extent(q.token, q.head, sh.tokens, sh.heads, d) * 2, out.data,
-                    extent(out.token, out.head, sh.tokens, sh.heads, d) * 2))
+    if (rows_meet(q.data, q.token, q.head, sh.heads, out.data, out.token, out.head, sh.heads, sh.tokens, d, 2))
         return fail(SPL_SAGE_ERR_INVALID, "%s: the output overlaps Q", call);
     float scale = 1.0f / sqrtf((float)d);
     if (opts) {

@@ -291,3 +291,15 @@ def test_read_outputs_over_one_another(calls):
         assert c.read(k=k, v=v) == 1 and text in c.why(), c.why()
     assert c.read(k=c.t(at, **both), v=c.t(at + 4 * d, **both)) != 0 and "overlap" not in c.why()
     assert c.read(k=c.t(at, token=2 * d, head=d), v=c.t(at + 2 * 10 * d, token=2 * d, head=d)) != 0 and "overlap" not in c.why()
+
+
+def test_outputs_between_the_rows_of_inputs(calls):
+    """Rotation and attention into heads beside their input's in one buffer: not an overlap."""
+    c, d = calls, calls.d
+    c.mem[1:] = [(-1 << 32) | d] + [-1] * 14  # an engine of device -1: no call gets past the check of the device
+    c.ws_mem[0] = (d << 32) | 0xffffffff
+    at, wide = 0x20000000, dict(token=16 * d, head=d)
+    for shift, fine in ((8 * d, True), (7 * d + 8, False), (-8 * d, True), (24 * d, True), (25 * d - 8, False)):
+        for call, arg in ((c.rope, "x"), (c.attend, "q")):
+            rc = call(**{arg: c.t(at, **wide), "out": c.t(at + 2 * shift, **wide)})
+            assert rc != 0 and ("overlaps" in c.why()) == (not fine), (arg, shift, c.why())
