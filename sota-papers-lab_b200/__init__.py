@@ -705,12 +705,14 @@ class SageAttention:
         return Kv4Workspace(self)
 
     def kv4_attend(self, ws: "Kv4Workspace", cache: "Kv4Cache", q, out, pages, kv_len, *, q_start=None,
-                   max_q: int = 1, causal: bool = True, window: int = 0, softmax_scale: float | None = None, lse=None):
+                   max_q: int | None = None, causal: bool = True, window: int = 0, softmax_scale: float | None = None, lse=None):
         """Attention of q bf16 [tokens][heads][head_dim] over the 4-bit cache
         (spl_sage_kv4_attend): pages int32 [batch][max_pages], kv_len int32
         [batch], q_start int32 [batch + 1] (None: one query per sequence), at
-        most max_q queries a sequence; writes out and, where given, lse f32
-        [tokens][heads]."""
+        most max_q queries a sequence (None: any number, which with q_start
+        takes the kernel for prompts where the tokens of all sequences
+        together are many: give it where it is known); writes out and, where
+        given, lse f32 [tokens][heads]."""
         torch = _torch()
         bf, t, h, c, b = _BF16, q.shape[0], q.shape[1], cache._c(self), kv_len.shape[0]
         cq, co = self._rows("Q", q, bf, t, h), self._rows("output", out, bf, t, h)
@@ -721,6 +723,8 @@ class SageAttention:
             raise SageError(ERR_INVALID, f"pages must be [batch][max_pages], got {list(pages.shape)}")
         if not 0 <= window <= 1 << 30:  # the struct's field would wrap
             raise SageError(ERR_INVALID, f"a window of {window} keys")
+        if max_q is None:
+            max_q = 1 if q_start is None else t
         sh = _Kv4Shape(b, h, t, max_q, pages.shape[1], int(causal), window)
         opts = None
         if softmax_scale is not None:

@@ -1343,3 +1343,15 @@ def test_append_with_q_in_place(engines, layout):
             eng.kv4_append(sage.Kv4Cache(pools[1], page, d), other["k"], other["v"], slots, rotary=r, positions=pos, q=q,
                            q_out=q)
     eng.engine_status()
+
+
+@pytest.mark.parametrize("rows", [4, 60])
+def test_attend_without_max_q_takes_any_number_of_queries(engines, rows):
+    """max_q is a bound that speeds a call up; left out, every query of every sequence is answered."""
+    d, eng, ws = 128, engines[128], engines["ws", 128]
+    b = Batch(d, 16, 8, 2, [300, 90, 200], [rows, 1, 2], seed=6)
+    b.fill(eng)
+    eng.kv4_attend(ws, sage.Kv4Cache(b.pool, 16, d), b.q, b.out, b.pages, b.kv_len, q_start=b.q_start, lse=b.lse)
+    eng.engine_status()
+    check_attend(b, "no max_q")
+    assert (b.out[sum(b.qn):] == 3.0).all()
