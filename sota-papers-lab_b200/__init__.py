@@ -1007,16 +1007,23 @@ class Rotary:
     (2p, 2p + 1) where interleaved (spl_sage_rotary)."""
 
     def __init__(self, table, rot_dim: int, interleaved: bool = False):
-        shape = table.shape
+        self.table, self.rot_dim, self.interleaved = table, rot_dim, interleaved
+        self._view()
+
+    def _view(self):
+        table, rot_dim, shape = self.table, self.rot_dim, self.table.shape
         if (not table.is_cuda or table.dtype != _torch().float32 or not table.is_contiguous() or len(shape) != 3
                 or shape[1] != rot_dim // 2 or shape[2] != 2):
             raise SageError(ERR_INVALID, f"a rotary table is a contiguous f32 CUDA tensor [positions][{rot_dim // 2}]"
                                          f"[2], got {table.dtype} {list(table.shape)} on {table.device}")
-        self.table, self.rot_dim, self.interleaved = table, rot_dim, interleaved
-        self._struct = _Rotary(table.data_ptr(), shape[0], rot_dim, int(interleaved))
+        self._at, self._size, self._device = table.data_ptr(), table.numel(), table.get_device()
+        self._struct = _Rotary(self._at, shape[0], rot_dim, int(self.interleaved))
 
     def _c(self, eng: "SageAttention") -> _Rotary:
-        if self.table.get_device() != eng.device:
+        t = self.table
+        if t.data_ptr() != self._at or t.numel() != self._size:  # set_ or resize_ moved it
+            self._view()
+        if self._device != eng.device:
             raise SageError(ERR_INVALID, f"the rotary table is on {self.table.device}, the engine on device {eng.device}")
         return self._struct
 
@@ -1030,17 +1037,22 @@ class Kv4Cache:
     contiguous; a view of every second page, say, is fine."""
 
     def __init__(self, pool, page_tokens: int, head_dim: int):
-        block = Kv4Cache.block_bytes(head_dim, page_tokens)
+        self.pool, self.page_tokens, self.head_dim = pool, page_tokens, head_dim
+        self._view()
+
+    def _view(self):
+        pool = self.pool
+        block = Kv4Cache.block_bytes(self.head_dim, self.page_tokens)
         shape, st = pool.shape, pool.stride()
         if (not pool.is_cuda or pool.dtype != _torch().uint8 or len(shape) != 3 or shape[2] != block or st[2] != 1
                 or (shape[1] > 1 and st[1] != block)):
             raise SageError(ERR_INVALID, f"a cache pool is a uint8 CUDA tensor [pages][kv_heads][{block}] with "
                                          f"contiguous pages, got {pool.dtype} {list(pool.shape)} with strides {st} on "
                                          f"{pool.device}")
-        self.pool, self.page_tokens, self.head_dim = pool, page_tokens, head_dim
         pages, heads = shape[0], shape[1]
         stride = st[0] if pages > 1 else heads * block
-        self._struct = _Kv4(pool.data_ptr(), pages, stride, page_tokens, heads)
+        self._at, self._size, self._device = pool.data_ptr(), pool.numel(), pool.get_device()
+        self._struct = _Kv4(self._at, pages, stride, self.page_tokens, heads)
 
     @staticmethod
     def block_bytes(head_dim: int, page_tokens: int) -> int:
@@ -1061,7 +1073,10 @@ class Kv4Cache:
         return Kv4Cache(torch.zeros(pages, kv_heads, block, dtype=torch.uint8, device="cuda"), page_tokens, head_dim)
 
     def _c(self, eng: "SageAttention") -> _Kv4:
-        if self.head_dim != eng.head_dim or self.pool.get_device() != eng.device:
+        t = self.pool
+        if t.data_ptr() != self._at or t.numel() != self._size:  # set_ or resize_ moved it
+            self._view()
+        if self.head_dim != eng.head_dim or self._device != eng.device:
             raise SageError(ERR_INVALID, f"the cache is for head dim {self.head_dim} on {self.pool.device}, the engine "
                                          f"for {eng.head_dim} on device {eng.device}")
         return self._struct

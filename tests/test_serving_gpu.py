@@ -1355,3 +1355,34 @@ def test_attend_without_max_q_takes_any_number_of_queries(engines, rows):
     eng.engine_status()
     check_attend(b, "no max_q")
     assert (b.out[sum(b.qn):] == 3.0).all()
+
+
+def test_tensors_that_moved_are_found_again(engines):
+    """A pool and a rotary table whose tensors got other memory (set_, a larger or smaller one) after they were wrapped:
+    the calls use what the tensors are now, or refuse it."""
+    d, page, eng = 128, 16, engines[128]
+    g = gen(3)
+    block = sage.Kv4Cache.block_bytes(d, page)
+    pools = [torch.zeros(n, 2, block, dtype=torch.uint8, device=DEV) for n in (4, 6, 2)]
+    tabs = [table(d, 50), table(d, 80, sage.RopeScaling.linear(2.0))]
+    pool, tab = pools[0].view_as(pools[0]).detach(), tabs[0].view_as(tabs[0]).detach()
+    cache, r = sage.Kv4Cache(pool, page, d), sage.Rotary(tab, d)
+    k, v, slots, pos = rand(g, 5, 2, d), rand(g, 5, 2, d), ints([0, 17, 35, 50, 63]), ints([1, 2, 3, 49, 30])
+    eng.kv4_append(cache, k, v, slots, rotary=r, positions=pos)
+    first = pools[0].clone()
+    pool.set_(pools[1])
+    tab.set_(tabs[1])
+    slots[4], pos[4] = 95, 79
+    eng.kv4_append(cache, k, v, slots, rotary=r, positions=pos)
+    want = torch.zeros_like(pools[1])
+    eng.kv4_append(sage.Kv4Cache(want, page, d), k, v, slots, rotary=sage.Rotary(tabs[1], d), positions=pos)
+    assert torch.equal(pools[1], want) and torch.equal(pools[0], first)
+    eng.engine_status()
+    pool.set_(pools[2])
+    eng.kv4_append(cache, k, v, slots, rotary=r, positions=pos)  # two pages: the other slots are out of range
+    with pytest.raises(sage.SageError, match="out of range"):
+        eng.engine_status()
+    pool.set_(torch.zeros(4, 2, block - 16, dtype=torch.uint8, device=DEV))
+    with pytest.raises(sage.SageError, match="cache pool"):
+        eng.kv4_append(cache, k, v, slots)
+    eng.engine_status()
