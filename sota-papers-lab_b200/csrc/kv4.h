@@ -47,9 +47,9 @@ struct RotaryArgs {
 
 // dtype: 0 bf16, 1 f16, 2 f32
 cudaError_t launch_rope(int d, int dtype, const Rows& x, const Rows& out, const RotaryArgs& r, int tokens, int heads,
-                        bool backward, uint32_t* err, cudaStream_t st);
+                        bool backward, int sms, uint32_t* err, cudaStream_t st);
 cudaError_t launch_kv4_append(int d, const Kv4Pool& pool, const Rows& q, const Rows& q_out, const Rows& k,
-                              const Rows& v, const RotaryArgs& r, const int* slots, int tokens, int q_heads,
+                              const Rows& v, const RotaryArgs& r, const int* slots, int tokens, int q_heads, int sms,
                               uint32_t* err, cudaStream_t st);
 cudaError_t launch_kv4_read(int d, const Kv4Pool& pool, const int* slots, const Rows& k, const Rows& v, int tokens,
                             uint32_t* err, cudaStream_t st);

@@ -238,7 +238,8 @@ int spl_sage_rope(spl_sage* s, int dtype, int64_t tokens, int64_t heads, spl_sag
         return fail(SPL_SAGE_ERR_INVALID, "%s: the output overlaps x without being x", call);
     if ((rc = check_device(call, s))) return rc;
     const cudaError_t e = sp::launch_rope(s->head_dim, dtype, {x.data, x.token, x.head}, {out.data, out.token, out.head},
-                                          r, (int)tokens, (int)heads, backward != 0, s->err, s->stream);
+                                          r, (int)tokens, (int)heads, backward != 0, s->sm_count, s->err,
+                                          s->stream);
     if (e != cudaSuccess) return cuda_fail(e, "launch rope");
     return SPL_SAGE_OK;
 }
@@ -280,7 +281,8 @@ int spl_sage_kv4_append(spl_sage* s, const spl_sage_kv4* cache, int64_t tokens, 
     if ((rc = check_device(call, s))) return rc;
     const cudaError_t e = sp::launch_kv4_append(
         s->head_dim, pool, {q.data, q.token, q.head}, {q_out.data, q_out.token, q_out.head}, {k.data, k.token, k.head},
-        {v.data, v.token, v.head}, r, slots, (int)tokens, (int)q_heads, s->err, s->stream);
+        {v.data, v.token, v.head}, r, slots, (int)tokens, (int)q_heads, s->sm_count, s->err,
+        s->stream);
     if (e != cudaSuccess) return cuda_fail(e, "launch the cache append");
     return SPL_SAGE_OK;
 }

@@ -229,8 +229,8 @@ __global__ void __launch_bounds__(APPEND_THREADS, 16) sp_kv4_append(const Kv4Poo
 
 template <int D>
 static cudaError_t append(const Kv4Pool& pool, const Rows& q, const Rows& q_out, const Rows& k, const Rows& v,
-                          const RotaryArgs& r, const int* slots, int tokens, int q_heads, uint32_t* err,
-                          cudaStream_t st) {
+                          const RotaryArgs& r, const int* slots, int tokens, int q_heads, int sms,
+                          uint32_t* err, cudaStream_t st) {
     constexpr int HL = 512 / D;
     // Two heads a thread, which share the angles, once that makes two rounds of
     // warps (append and read back, two heads against one: 8192 tokens of 32 / 8
@@ -239,7 +239,7 @@ static cudaError_t append(const Kv4Pool& pool, const Rows& q, const Rows& q_out,
     constexpr int MANY = 2;
     auto blocks = [](int heads, int per) { return (heads + per - 1) / per; };
     const bool many =
-        (long long)tokens * (blocks(q_heads, MANY * HL) + 2 * blocks(pool.kv_heads, MANY * HL)) >= 148 * 64;
+        (long long)tokens * (blocks(q_heads, MANY * HL) + 2 * blocks(pool.kv_heads, MANY * HL)) >= sms * 64;
     const int per = many ? MANY * HL : HL, qb = blocks(q_heads, per), rb = qb + 2 * blocks(pool.kv_heads, per);
     const unsigned grid = (unsigned)(((long long)tokens * rb + APPEND_THREADS / 32 - 1) / (APPEND_THREADS / 32));
     return launch_after_previous(many ? sp_kv4_append<D, MANY> : sp_kv4_append<D, 1>, dim3(grid), dim3(APPEND_THREADS), 0,
@@ -247,10 +247,10 @@ static cudaError_t append(const Kv4Pool& pool, const Rows& q, const Rows& q_out,
 }
 
 cudaError_t launch_kv4_append(int d, const Kv4Pool& pool, const Rows& q, const Rows& q_out, const Rows& k,
-                              const Rows& v, const RotaryArgs& r, const int* slots, int tokens, int q_heads,
+                              const Rows& v, const RotaryArgs& r, const int* slots, int tokens, int q_heads, int sms,
                               uint32_t* err, cudaStream_t st) {
-    return d == 64 ? append<64>(pool, q, q_out, k, v, r, slots, tokens, q_heads, err, st)
-                   : append<128>(pool, q, q_out, k, v, r, slots, tokens, q_heads, err, st);
+    return d == 64 ? append<64>(pool, q, q_out, k, v, r, slots, tokens, q_heads, sms, err, st)
+                   : append<128>(pool, q, q_out, k, v, r, slots, tokens, q_heads, sms, err, st);
 }
 
 // The values at given slots, zero + scale * n rounded once to bf16.  A thread

@@ -65,13 +65,13 @@ __global__ void __launch_bounds__(256) sp_rope(const Rows x, const Rows out, con
 
 template <int D, int DT>
 static cudaError_t rope(const Rows& x, const Rows& out, const RotaryArgs& r, int tokens, int heads, bool backward,
-                        uint32_t* err, cudaStream_t st) {
+                        int sms, uint32_t* err, cudaStream_t st) {
     constexpr int HL = 512 / D;  // heads a warp covers at once
     // Several heads a thread once that still leaves every SM a few warps: 4 of
     // a 16-bit type (8192 x 40 x 128 bf16: 28.7 us, 5.99 TB/s, with 1 41.6), 2
     // in f32, whose loads are twice as many (4099 x 32 x 64: 14.5 us, with 4 16.3).
     constexpr int MANY = DT == 2 ? 2 : 4;
-    const bool many = (long long)tokens * ((heads + MANY * HL - 1) / (MANY * HL)) >= 148 * 16;
+    const bool many = (long long)tokens * ((heads + MANY * HL - 1) / (MANY * HL)) >= sms * 16;
     const int per = many ? MANY : 1, hb = (heads + per * HL - 1) / (per * HL);
     const long long warps = (long long)tokens * hb;
     const unsigned grid = (unsigned)((warps + 7) / 8);
@@ -80,14 +80,14 @@ static cudaError_t rope(const Rows& x, const Rows& out, const RotaryArgs& r, int
 }
 
 cudaError_t launch_rope(int d, int dtype, const Rows& x, const Rows& out, const RotaryArgs& r, int tokens, int heads,
-                        bool backward, uint32_t* err, cudaStream_t st) {
+                        bool backward, int sms, uint32_t* err, cudaStream_t st) {
     if (d == 64)
-        return dtype == 0   ? rope<64, 0>(x, out, r, tokens, heads, backward, err, st)
-               : dtype == 1 ? rope<64, 1>(x, out, r, tokens, heads, backward, err, st)
-                            : rope<64, 2>(x, out, r, tokens, heads, backward, err, st);
-    return dtype == 0   ? rope<128, 0>(x, out, r, tokens, heads, backward, err, st)
-           : dtype == 1 ? rope<128, 1>(x, out, r, tokens, heads, backward, err, st)
-                        : rope<128, 2>(x, out, r, tokens, heads, backward, err, st);
+        return dtype == 0   ? rope<64, 0>(x, out, r, tokens, heads, backward, sms, err, st)
+               : dtype == 1 ? rope<64, 1>(x, out, r, tokens, heads, backward, sms, err, st)
+                            : rope<64, 2>(x, out, r, tokens, heads, backward, sms, err, st);
+    return dtype == 0   ? rope<128, 0>(x, out, r, tokens, heads, backward, sms, err, st)
+           : dtype == 1 ? rope<128, 1>(x, out, r, tokens, heads, backward, sms, err, st)
+                        : rope<128, 2>(x, out, r, tokens, heads, backward, sms, err, st);
 }
 
 }  // namespace sp
