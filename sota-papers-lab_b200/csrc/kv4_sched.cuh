@@ -286,42 +286,57 @@ __device__ __forceinline__ void join_tile(const Kv4Attend& a, const Seq& s, int 
     auto sync = [] { named_bar(1, THREADS); };
     constexpr int LANES = D / 4, TEAMS = THREADS / LANES;
     const int lane = threadIdx.x % LANES, team = threadIdx.x / LANES;
-    if (c1 - c0 < 4 && cols > TEAMS) {
-        // few pieces of many columns (a prompt's tile cut at a CTA's border):
-        // four columns a team at a time, their loads all under way together
-        for (int first = team; first < cols; first += 4 * TEAMS) {
-            float2 ml[4][4];
-            float4 y[4][4];
+    if (cols > TEAMS) {
+        // many columns (a prompt's tile): NC a team at a time, NP pieces of
+        // each in one go, whose loads are all under way together
+        constexpr int NC = 4, NP = 3;
+        for (int first = team; first < cols; first += NC * TEAMS) {
+            float m[NC], sum[NC];
+            float4 v[NC];
 #pragma unroll
-            for (int k = 0; k < 4; k++)
+            for (int k = 0; k < NC; k++) {
+                m[k] = -INFINITY;
+                sum[k] = 0.f;
+                v[k] = make_float4(0.f, 0.f, 0.f, 0.f);
+            }
+            for (int b = c0; b <= c1; b += NP) {
+                float2 ml[NC][NP];
+                float4 y[NC][NP];
 #pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    const int col = first + k * TEAMS, c = c0 + i;
-                    ml[k][i] = make_float2(-INFINITY, 0.f);
-                    y[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
-                    if (c <= c1 && col < cols) {
-                        const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
-                        ml[k][i] = __ldcg(&a.part_ml[slot]);
-                        y[k][i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
+                for (int k = 0; k < NC; k++)
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        const int col = first + k * TEAMS, c = b + i;
+                        ml[k][i] = make_float2(-INFINITY, 0.f);
+                        y[k][i] = make_float4(0.f, 0.f, 0.f, 0.f);
+                        if (c <= c1 && col < cols) {
+                            const long long slot = (long long)(2 * c + (c == c0)) * COLS + col;
+                            ml[k][i] = __ldcg(&a.part_ml[slot]);
+                            y[k][i] = __ldcg((const float4*)(a.part_o + slot * D + 4 * lane));
+                        }
+                    }
+#pragma unroll
+                for (int k = 0; k < NC; k++) {
+                    const float old = m[k];
+#pragma unroll
+                    for (int i = 0; i < NP; i++) m[k] = fmaxf(m[k], ml[k][i].x);
+                    const float ref = m[k] == -INFINITY ? 0.f : m[k], f0 = ex2(old - ref);
+                    sum[k] *= f0;
+                    v[k].x *= f0; v[k].y *= f0; v[k].z *= f0; v[k].w *= f0;
+#pragma unroll
+                    for (int i = 0; i < NP; i++) {
+                        float f = ex2(ml[k][i].x - ref);
+                        sum[k] = fmaf(f, ml[k][i].y, sum[k]);
+                        if (MEANS) f *= ml[k][i].y;
+                        v[k].x = fmaf(f, y[k][i].x, v[k].x); v[k].y = fmaf(f, y[k][i].y, v[k].y);
+                        v[k].z = fmaf(f, y[k][i].z, v[k].z); v[k].w = fmaf(f, y[k][i].w, v[k].w);
                     }
                 }
-#pragma unroll
-            for (int k = 0; k < 4; k++) {
-                if (first + k * TEAMS >= cols) break;
-                const float m = fmaxf(fmaxf(ml[k][0].x, ml[k][1].x), fmaxf(ml[k][2].x, ml[k][3].x));
-                const float ref = m == -INFINITY ? 0.f : m;
-                float sum = 0.f;
-                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-                for (int i = 0; i < 4; i++) {
-                    float f = ex2(ml[k][i].x - ref);
-                    sum = fmaf(f, ml[k][i].y, sum);
-                    if (MEANS) f *= ml[k][i].y;
-                    v.x = fmaf(f, y[k][i].x, v.x); v.y = fmaf(f, y[k][i].y, v.y);
-                    v.z = fmaf(f, y[k][i].z, v.z); v.w = fmaf(f, y[k][i].w, v.w);
-                }
-                put_row<D>(a, s, head, n0 + first + k * TEAMS, 4 * lane, v, ref, sum);
             }
+#pragma unroll
+            for (int k = 0; k < NC; k++)
+                if (first + k * TEAMS < cols)
+                    put_row<D>(a, s, head, n0 + first + k * TEAMS, 4 * lane, v[k], m[k] == -INFINITY ? 0.f : m[k], sum[k]);
         }
         sync();
         return;
