@@ -33,8 +33,8 @@
 // own running maximum and sums; the warps meet once per tile.  Row maxima are
 // looked at by vote and only recomputed when one grows.
 //
-// Measured, 32 / 8 heads, D = 128: one sequence of 131072 tokens (151 MB) 44 us,
-// 64 of up to 8192 (371 MB) 93 us; another 151 MB add 29 us (5.2 TB/s, where a
+// Measured, 32 / 8 heads, D = 128: one sequence of 131072 tokens (151 MB) 45 us,
+// 64 of up to 8192 (371 MB) 94.5 us; another 151 MB add 29 us (5.2 TB/s, where a
 // copy reaches 6.45; the issue slots are 3/4 busy).  The rest is a call's start
 // (3 us from the lengths to the first loads), the ends of pieces (about 4 us
 // each, beside the SM's other CTA) and the join (4 us).  One sequence of 1000
@@ -54,7 +54,7 @@ constexpr int AT_WARPS = 8, AT_STEP = 32, AT_UNIT = 128;
 // 16.8, 9000: 12.6 and 18.8).
 constexpr int AT_LEAST = 2;
 // Units that a tile's start and end count for beside its own (two CTAs on an SM
-// and one): 64 sequences of up to 8192 tokens, 32 / 8 heads, D = 128, take 93 us
+// and one), times before the scales were checked: 64 sequences of up to 8192 tokens, 32 / 8 heads, D = 128, take 93 us
 // instead of 102 with none (93.8 with 6, 97.6 with 11), 16 of up to 4096, 16 / 16
 // heads, D = 64, 21.8 instead of 28.9; 20 rows in two tiles 40.4 instead of 42
 // (41.2 with 4 and 8).
@@ -862,9 +862,12 @@ cudaError_t launch_kv4_attend(int d, const Kv4Attend& a, int sms, bool alone, cu
     const int rows = a.max_q * a.group;
     // Above 128 rows the tensor-core kernel with a tile of up to 256 rows, up
     // to there this one's tiles of 16 (which read the cache again from the L2).
-    // 8 sequences, window 8192, 32 / 8 heads, D = 128, us here and there: 20
-    // rows 43 and 105, 64 rows 65 and 108, 128 rows 110 and 113, 256 rows 201
-    // and 131; one sequence of 2000 tokens, 128 rows: 19 and 54.
+    // 32 / 8 heads, D = 128, us here and there: 8 sequences, window 8192: 20
+    // rows 41 and 110, 64 rows 65 and 114, 128 rows 110 and 119, 160 rows 121
+    // and 127, 200 rows 185 and 133, 256 rows 200 and 137; one sequence of 32000
+    // tokens: 128 rows 97 and 88.  With little work the border lies higher (one
+    // sequence of 2000 tokens: 256 rows 26 and 45, 1024 rows 71 and 50): lengths
+    // are not known here, and the rule does not guess them.
     if (rows > 128) return launch_kv4_prompt(d, a, sms, st);
     if (d == 64) return rows <= 8 ? attend<64, 1>(a, sms, alone, st) : attend<64, 2>(a, sms, alone, st);
     return rows <= 8 ? attend<128, 1>(a, sms, alone, st) : attend<128, 2>(a, sms, alone, st);

@@ -37,7 +37,7 @@
 // ever rescaled.
 //
 // Measured: 2 x 2048 query tokens on up to 8192 cached ones, 32 / 8 heads, D =
-// 128 (382 GFLOP), 549 us, 695 TFLOP/s, 0.42 of a large bf16 product's rate.
+// 128 (382 GFLOP), 566 us, 675 TFLOP/s, 0.41 of a large bf16 product's rate.
 // No unit bounds it: without the exponentials it took 519 of then 562 us,
 // without the products 520, without the unpacking arithmetic 549; the chain
 // from S to the P that waits for it does.
@@ -54,7 +54,7 @@ namespace sp {
 constexpr int PR_ROWS = 256, PR_KEYS = 128;
 constexpr int PR_LEAST = 4;  // key tiles a CTA takes at least: a piece's start, end and joining cost as much as several
 constexpr uint32_t R_BELOW = 4;  // how far a tile's R may lie below the one that a row's O refers to: P of 2^-28 is not lost
-constexpr int PR_BEGIN = 3;  // what a tile's start and end count for when they are shared out (549 us instead of 575, 551 with 6)
+constexpr int PR_BEGIN = 3;  // what a tile's start and end count for when they are shared out (549 us instead of 575, 551 with 6, then)
 constexpr int PR_SOFTMAX = 8, PR_UNPACK = 8, PR_MMA_WARP = 16, PR_HELP_WARP = 17, PR_THREADS = 20 * 32;
 // Registers a thread: what the block is launched with, and what the
 // warpgroups make of them (raising more than there are would wait for ever).

@@ -3,7 +3,7 @@
 // the pairs); backward: y = R(position)^T x.
 //
 // Bound by memory: every element is read and written once; the 8192-token bf16
-// case runs at 0.93 of the measured copy rate.  A thread keeps
+// case runs at 0.91 of the measured copy rate.  A thread keeps
 // the cosines and sines of its 8 pairs in registers and applies them to HPT
 // heads of its token, whose loads are all issued before the first is used:
 // with one head a thread the table (64 bytes for 32 bytes of bf16 channels)
@@ -68,7 +68,7 @@ static cudaError_t rope(const Rows& x, const Rows& out, const RotaryArgs& r, int
                         int sms, uint32_t* err, cudaStream_t st) {
     constexpr int HL = 512 / D;  // heads a warp covers at once
     // Several heads a thread once that still leaves every SM a few warps: 4 of
-    // a 16-bit type (8192 x 40 x 128 bf16: 28.7 us, 5.99 TB/s, with 1 41.6), 2
+    // a 16-bit type (8192 x 40 x 128 bf16: 29.2 us, 5.89 TB/s, with 1 41.6), 2
     // in f32, whose loads are twice as many (4099 x 32 x 64: 14.5 us, with 4 16.3).
     constexpr int MANY = DT == 2 ? 2 : 4;
     const bool many = (long long)tokens * ((heads + MANY * HL - 1) / (MANY * HL)) >= sms * 16;
