@@ -958,6 +958,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                     t = sm_far.t;
                     marks = sm_far.marks;
                     if (!(ok = sm_far.ok)) break;
+                    // (the smallest that fitted before may be too large for the new R)
+#pragma unroll
+                    for (int i = 0; i < NG; i++) kp[i] = keep & 256u ? kp[i] : 0u;
+#pragma unroll
+                    for (int i = 0; i < 8; i++) vp[i] = keep >> i & 1 ? vp[i] : 0u;
                 }
                 if (!done) {
                     const int E = sm_far.E;

@@ -1386,3 +1386,35 @@ def test_tensors_that_moved_are_found_again(engines):
     with pytest.raises(sage.SageError, match="cache pool"):
         eng.kv4_append(cache, k, v, slots)
     eng.engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("rows", [1, 5, 90])
+@pytest.mark.parametrize("value", [0.0, 2.5, -7.0e30])
+def test_attend_constant_caches(engines, d, rows, value):
+    """No group has a scale: each key's V is its zero, all keys weigh the same, the mean is exact."""
+    b = Batch(d, 32, 4, 2, [800, 3], [rows, 1], seed=rows, tail_rows=0)
+    b.k.fill_(0.375)
+    b.v.fill_(value)
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d], causal=False)
+    want = torch.tensor(value).bfloat16().to(DEV)
+    # sums of equal numbers in f32, up to 800 of them: 2^-24 each, then bf16's rounding of a bf16 number
+    assert ((b.out - want).abs() <= 2.0 ** -7 * want.abs()).all()
+    score = (b.q.float().sum(-1) * 0.375).double() * d ** -0.5
+    n = torch.cat([torch.full((rows,), 800.0), torch.full((1,), 3.0)]).to(DEV).double()[:, None]
+    assert ((b.lse.double() - score - n.log()).abs() <= 1e-4).all()
+    engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("scale", [2.0 ** -30, 2.0 ** -12, 2.0 ** 9, 2.0 ** 40])
+@pytest.mark.parametrize("rows", [1, 90])
+def test_attend_short_sequences_of_any_size_of_values(engines, d, scale, rows):
+    """All keys of one magnitude, far from one, in sequences that end within a tile."""
+    b = Batch(d, 16, 4, 2, [3, 130, 17, 90, 257], [min(rows, 3), rows, min(rows, 17), rows, rows], seed=rows, tail_rows=0)
+    b.k, b.v = (b.k.float() * min(scale, 8.0)).bfloat16(), (b.v.float() * scale).bfloat16()
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    check_attend(b, "size")
+    engines[d].engine_status()
