@@ -597,7 +597,7 @@ typedef struct {
  * ones to f32's rounding, sums f32; a probability times its V scale is rounded
  * to f16 (2^-11; below 2^-26 of the row's largest nothing may be left of it).  With
  * max_q * heads / kv_heads above 128 (prompts) each V value and each probability
- * is (a value by 2^-10 of the largest that its group's scale can give where it
+ * is (a value by 2^-12 of the largest that its group's scale can give where it
  * is small, a probability below 2^-28 counts as 0), and where the scales of one
  * key's two groups of K are more than 2^8 apart, the smaller one's products are
  * rounded by 2^-17 of the larger scale.  A row's precision depends on the keys
