@@ -272,7 +272,8 @@ __device__ __forceinline__ bool pick_keys(PromptTile& tile, FarTile& far, int gr
         int top = ANY;
 #pragma unroll
         for (int b = 0; b < 4; b++) top = max(top, open >> b & 1 ? E[b] : ANY);
-        top_E = max(__reduce_max_sync(0xffffffffu, top), -100);
+        top_E = __reduce_max_sync(0xffffffffu, top);
+        if (top_E == ANY) top_E = far.E;
         if (far.E > top_E && far.E <= top_E + 2) top_E = far.E;  // (no need to go up and down)
         top = ANY;
 #pragma unroll
@@ -283,7 +284,8 @@ __device__ __forceinline__ bool pick_keys(PromptTile& tile, FarTile& far, int gr
                 for (int gr = 0; gr < 2; gr++)
                     if (left[gr] >> b & 1) top = max(top, R[b][gr]);
             }
-        top_R = max(__reduce_max_sync(0xffffffffu, top), -100);
+        top_R = __reduce_max_sync(0xffffffffu, top);
+        if (top_R == ANY) top_R = far.R;
         if (far.R > top_R && far.R <= top_R + 2) top_R = far.R;
 #pragma unroll
         for (int gr = 0; gr < 2; gr++) {
@@ -621,9 +623,11 @@ __global__ void __launch_bounds__(PR_THREADS, 1) sp_kv4_prompt(const __grid_cons
                         bool far_R = (uint32_t)(R_ref - R) > R_BELOW;
                         // (at most 7, so P at most 2^15; below -40 nothing is left of it in f16)
                         int shift = min(max(7 + R - R_ref, -40), 7);
-                        // what S is multiplied by: softmax scale times 2^(E - up), in two steps (either may be far from 1)
-                        const int e = tile.E - up_row;
-                        const float f = fminf(fmaxf(a.c * exp2i(e >> 1) * exp2i(e - (e >> 1)), 1e-37f), 3e38f);
+                        // What S is multiplied by: softmax scale times 2^(E - up), in two steps (either may be far from 1).
+                        // (At least 2^-87, where f is at least 2^-120 whatever the scale: S is below 2^27, and what is left
+                        // of a score there is nothing.  The reference has to be in the same units.)
+                        const int e = max(tile.E - up_row, -87);
+                        const float f = fminf(a.c * exp2i(e >> 1) * exp2i(e - (e >> 1)), 3e38f);
                         float m_s = m_ref * exp2i(-e >> 1) * exp2i(-e - (-e >> 1));  // the reference in S's units
 #pragma unroll 1
                         for (int h = 0; h < 2; h++) {

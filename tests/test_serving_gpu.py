@@ -1418,3 +1418,18 @@ def test_attend_short_sequences_of_any_size_of_values(engines, d, scale, rows):
     b.attend(engines[d], engines["ws", d])
     check_attend(b, "size")
     engines[d].engine_status()
+
+
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("size", [1.0, 1e-6, 1e-20])
+@pytest.mark.parametrize("rows", [4, 90])
+@pytest.mark.parametrize("key", [0.0, 0.25, 1e-25])
+def test_attend_constant_keys_and_values_among_others(engines, d, size, rows, key):
+    """Every fourth key constant (or nothing), its value too, small queries: it weighs what it should beside the others."""
+    b = Batch(d, 16, 4, 2, [600, 130, 47], [rows, rows, min(rows, 47)], seed=rows, tail_rows=0)
+    b.k[::4], b.v[::4] = key, 1.0
+    b.q = (b.q.float() * size).bfloat16()
+    b.fill(engines[d])
+    b.attend(engines[d], engines["ws", d])
+    check_attend(b, "constant")
+    engines[d].engine_status()
