@@ -654,7 +654,7 @@ class SageAttention:
 
     def _index(self, what: str, t, shape: tuple) -> int:
         """The address of an int32 CUDA array of this engine's device."""
-        if t.get_device() != self.device or t.dtype != _torch().int32 or t.shape != shape or not t.is_contiguous():
+        if t.get_device() != self.device or t.dtype != _I32 or t.shape != shape or not t.is_contiguous():
             raise SageError(ERR_INVALID, f"{what} must be a contiguous int32 tensor {list(shape)} on device "
                                          f"{self.device}, got {t.dtype} {list(t.shape)} on {t.device}")
         return t.data_ptr()
@@ -945,15 +945,16 @@ class RopeTable:
 _TORCH = None
 _ROPE_TYPES: dict = {}  # torch types of SageAttention.rope -> SPL_SAGE_BF16, _F16, _F32
 _BF16: tuple = ()
+_I32 = _F32 = _U8 = None
 
 
 def _torch():
     """torch, imported by the first call that takes tensors."""
-    global _TORCH, _BF16
+    global _TORCH, _BF16, _I32, _F32, _U8
     if _TORCH is None:
         import torch
         _ROPE_TYPES.update({torch.bfloat16: 0, torch.float16: 1, torch.float32: 2})
-        _BF16 = (torch.bfloat16,)
+        _BF16, _I32, _F32, _U8 = (torch.bfloat16,), torch.int32, torch.float32, torch.uint8
         _TORCH = torch
     return _TORCH
 
@@ -1012,7 +1013,9 @@ class Rotary:
 
     def _view(self):
         table, rot_dim, shape = self.table, self.rot_dim, self.table.shape
-        if (not table.is_cuda or table.dtype != _torch().float32 or not table.is_contiguous() or len(shape) != 3
+        if _F32 is None:
+            _torch()
+        if (not table.is_cuda or table.dtype != _F32 or not table.is_contiguous() or len(shape) != 3
                 or shape[1] != rot_dim // 2 or shape[2] != 2):
             raise SageError(ERR_INVALID, f"a rotary table is a contiguous f32 CUDA tensor [positions][{rot_dim // 2}]"
                                          f"[2], got {table.dtype} {list(table.shape)} on {table.device}")
@@ -1042,9 +1045,11 @@ class Kv4Cache:
 
     def _view(self):
         pool = self.pool
-        block = Kv4Cache.block_bytes(self.head_dim, self.page_tokens)
+        block = _KV4_BLOCKS.get((self.head_dim, self.page_tokens)) or Kv4Cache.block_bytes(self.head_dim, self.page_tokens)
         shape, st = pool.shape, pool.stride()
-        if (not pool.is_cuda or pool.dtype != _torch().uint8 or len(shape) != 3 or shape[2] != block or st[2] != 1
+        if _U8 is None:
+            _torch()
+        if (not pool.is_cuda or pool.dtype != _U8 or len(shape) != 3 or shape[2] != block or st[2] != 1
                 or (shape[1] > 1 and st[1] != block)):
             raise SageError(ERR_INVALID, f"a cache pool is a uint8 CUDA tensor [pages][kv_heads][{block}] with "
                                          f"contiguous pages, got {pool.dtype} {list(pool.shape)} with strides {st} on "
