@@ -594,7 +594,7 @@ typedef struct {
  * pages wholly before every query's window are not looked at).  A query that
  * sees no key gives zeros and an lse of -infinity.  q is bf16 and already
  * rotated; K and V are the cached values, scores and lse those of the exact
- * ones to f32's rounding, sums f32; a probability times its V scale is rounded
+ * ones to f32's rounding (prompts: to 2^-19 of what a score adds up), sums f32; a probability times its V scale is rounded
  * to f16 (2^-11; below 2^-26 of the row's largest nothing may be left of it).  With
  * max_q * heads / kv_heads above 128 (prompts) each V value and each probability
  * is (a value by 2^-12 of the largest that its group's scale can give where it

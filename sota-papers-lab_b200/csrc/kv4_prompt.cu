@@ -22,8 +22,8 @@
 // scaled by a power of two 2^-E; the rest of the value, c = zero + 8 scale, is
 // constant per group of 64 channels and enters through 16 more channels, as two
 // f16 terms times two f16 terms of the row's sum over the group (an error below
-// 2^-20 of that product).  So S is that of the exact cached values to f32's
-// rounding, and lse with it, where f16 values of K would put a row's lse off by
+// 2^-20 of that product, or 2^-19 of the key's largest value times the sum).  So S
+// is that of the exact cached values to about f32's rounding, and lse with it, where f16 values of K would put a row's lse off by
 // 1e-4 and more.  Each row of Q is scaled by a power of two of its own.
 // V: zero + scale * n, scaled by a power of two 2^-R, rounded to f16 (2^-11 of
 // itself, or 2^-25 of 2^R where that is more); P, times 2^7 and what R differs
@@ -37,7 +37,7 @@
 // ever rescaled.
 //
 // Measured: 2 x 2048 query tokens on up to 8192 cached ones, 32 / 8 heads, D =
-// 128 (382 GFLOP), 566 us, 675 TFLOP/s, 0.41 of a large bf16 product's rate.
+// 128 (382 GFLOP), 569 us, 671 TFLOP/s, 0.41 of a large bf16 product's rate.
 // No unit bounds it: without the exponentials it took 519 of then 562 us,
 // without the products 520, without the unpacking arithmetic 549; the chain
 // from S to the P that waits for it does.
@@ -203,10 +203,11 @@ struct __align__(16) PromptTile {
 // exact then: 8 bits of scale, 3 of n - 8 above f16's 2^-24), V's from
 // 2^-V_WIDE (its values are off by 2^-12 of the largest that the smallest such
 // scale can give; with 2^-10 instead, values at that end left the output off by
-// 0.0019 of itself instead of 0.0017).  Any other tile goes to the helper, which finds E and R for
-// it; where its keys are too far apart for one pair, or not finite, it works on
-// the tile in turns, each with the keys whose magnitudes go together and all
-// others hidden, so that no key takes precision from the rows that do not see it.
+// 0.0019 of itself instead of 0.0017).  Any other tile goes to the helper, which
+// finds E and R for it; where its keys are too far apart for one pair, or their V
+// is not finite, it works on the tile in turns, each with the keys whose
+// magnitudes go together and all others hidden, so that no key takes precision
+// from the rows that do not see it.
 constexpr int K_WIDE = 8, V_WIDE = 8;
 // E and R for a scale and zero (bf16 bits, zero in the upper half).  K: scales
 // below 2^-8, c below 2^6; V: scales below 2^-8, zeros below 2^13.
