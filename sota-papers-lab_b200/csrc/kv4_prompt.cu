@@ -23,8 +23,9 @@
 // constant per group of 64 channels and enters through 16 more channels, as two
 // f16 terms times two f16 terms of the row's sum over the group (an error below
 // 2^-20 of that product, or 2^-19 of the key's largest value times the sum).  So S
-// is that of the exact cached values to about f32's rounding, and lse with it, where f16 values of K would put a row's lse off by
-// 1e-4 and more.  Each row of Q is scaled by a power of two of its own.
+// is that of the exact cached values to about f32's rounding, and lse with it,
+// where f16 values of K would put a row's lse off by 1e-4 and more.  Each row of
+// Q is scaled by a power of two of its own.
 // V: zero + scale * n, scaled by a power of two 2^-R, rounded to f16 (2^-11 of
 // itself, or 2^-25 of 2^R where that is more); P, times 2^7 and what R differs
 // from the R that the row's O refers to, rounded to f16 likewise; sums in f32.
